@@ -24,6 +24,17 @@ __device__ __forceinline__ void raise_status(unsigned int bits) {
   atomicOr(&g_device_status, bits);
 }
 
+// Parent of node i as the kernels use it: an index that is not below i (or is
+// below -1) would make a cycle, so it is reported and the node becomes a root.
+__device__ __forceinline__ int tree_parent(const int32_t* parents, int i) {
+  const int a = parents[i];
+  if (a < -1 || a >= i) {
+    raise_status(CIE_DEV_BAD_TREE);
+    return -1;
+  }
+  return a;
+}
+
 // Upper bound for any single wait inside a kernel (nanoseconds). Pipeline
 // waits (a role waiting for another role's data or a free stage) read the
 // per-device value g_wait_limit_ns, which starts at this default and can be

@@ -121,8 +121,10 @@ __global__ void __launch_bounds__(256) rope_append_kernel(
     uint8_t* __restrict__ k_pool, uint8_t* __restrict__ v_pool,
     const int32_t* __restrict__ tables, const int32_t* __restrict__ start_pos, int L, int Hkv,
     int d, int num_blocks, int block_size, int max_blocks, int64_t s_b, int64_t s_l, int64_t s_h,
-    const float* __restrict__ cos, const float* __restrict__ sin, int max_pos) {
-  // grid.y = sequence; one thread = one 8-pair group of one (token, head) row
+    const float* __restrict__ cos, const float* __restrict__ sin, int max_pos,
+    const int32_t* __restrict__ parents, int64_t par_sb) {
+  // grid.y = sequence; one thread = one 8-pair group of one (token, head) row.
+  // parents: the tokens are the nodes of a tree, rotated at their depth in it
   const int half = d / 2;
   const int groups = half / 8;
   const int b = blockIdx.y;
@@ -148,7 +150,14 @@ __global__ void __launch_bounds__(256) rope_append_kernel(
     const uint4 x2 = *reinterpret_cast<const uint4*>(k_new + src_off + half * 2 + gi * 16);
     uint4 y1 = x1, y2 = x2;
     if (cos != nullptr) {
-      const int rp = clamp_pos(pos, max_pos);
+      int at = pos;
+      if (parents != nullptr) {
+        at = start;
+        for (int j = tree_parent(parents + b * par_sb, i); j >= 0;
+             j = tree_parent(parents + b * par_sb, j))  // indices only fall: ends
+          ++at;
+      }
+      const int rp = clamp_pos(at, max_pos);
       rotate8<BF16>(x1, x2, cos + static_cast<int64_t>(rp) * half + gi * 8,
                     sin + static_cast<int64_t>(rp) * half + gi * 8, y1, y2);
     }
@@ -256,11 +265,12 @@ extern "C" int cie_rope(const void* x, void* y, int B, int H, int L, int d,
                      rope_cos, rope_sin, rope_max_pos, reinterpret_cast<cudaStream_t>(stream));
 }
 
-extern "C" int cie_rope_append(const void* k_new, const void* v_new, void* k_pool, void* v_pool,
-                               const int32_t* block_tables, const int32_t* start_pos, int B, int L,
-                               int Hkv, int d, int num_blocks, int block_size, int max_blocks,
-                               const int64_t* kv_strides, int dtype, const float* rope_cos,
-                               const float* rope_sin, int rope_max_pos, void* stream) {
+static int rope_append_impl(const void* k_new, const void* v_new, void* k_pool, void* v_pool,
+                            const int32_t* block_tables, const int32_t* start_pos,
+                            const int32_t* parents, int64_t parents_stride_b, int B, int L,
+                            int Hkv, int d, int num_blocks, int block_size, int max_blocks,
+                            const int64_t* kv_strides, int dtype, const float* rope_cos,
+                            const float* rope_sin, int rope_max_pos, void* stream) {
   CIE_CHECK_ARG(k_new && v_new && k_pool && v_pool && block_tables && start_pos && kv_strides,
                 "cie_rope_append: null pointer");
   CIE_CHECK_ARG(B >= 0 && L >= 0 && Hkv > 0, "cie_rope_append: bad shape");
@@ -293,15 +303,40 @@ extern "C" int cie_rope_append(const void* k_new, const void* v_new, void* k_poo
         reinterpret_cast<const uint8_t*>(k_new), reinterpret_cast<const uint8_t*>(v_new),
         reinterpret_cast<uint8_t*>(k_pool), reinterpret_cast<uint8_t*>(v_pool), block_tables,
         start_pos, L, Hkv, d, num_blocks, block_size, max_blocks, kv_strides[0], kv_strides[1],
-        kv_strides[2], rope_cos, rope_sin, rope_max_pos);
+        kv_strides[2], rope_cos, rope_sin, rope_max_pos, parents, parents_stride_b);
   else
     rope_append_kernel<false><<<grid, threads, 0, st>>>(
         reinterpret_cast<const uint8_t*>(k_new), reinterpret_cast<const uint8_t*>(v_new),
         reinterpret_cast<uint8_t*>(k_pool), reinterpret_cast<uint8_t*>(v_pool), block_tables,
         start_pos, L, Hkv, d, num_blocks, block_size, max_blocks, kv_strides[0], kv_strides[1],
-        kv_strides[2], rope_cos, rope_sin, rope_max_pos);
+        kv_strides[2], rope_cos, rope_sin, rope_max_pos, parents, parents_stride_b);
   CIE_CHECK_LAUNCH("rope_append_kernel");
   return CIE_OK;
+}
+
+extern "C" int cie_rope_append(const void* k_new, const void* v_new, void* k_pool, void* v_pool,
+                               const int32_t* block_tables, const int32_t* start_pos, int B, int L,
+                               int Hkv, int d, int num_blocks, int block_size, int max_blocks,
+                               const int64_t* kv_strides, int dtype, const float* rope_cos,
+                               const float* rope_sin, int rope_max_pos, void* stream) {
+  return rope_append_impl(k_new, v_new, k_pool, v_pool, block_tables, start_pos, nullptr, 0, B, L,
+                          Hkv, d, num_blocks, block_size, max_blocks, kv_strides, dtype, rope_cos,
+                          rope_sin, rope_max_pos, stream);
+}
+
+extern "C" int cie_rope_append_tree(const void* k_new, const void* v_new, void* k_pool,
+                                    void* v_pool, const int32_t* block_tables,
+                                    const int32_t* start_pos, const int32_t* parents,
+                                    int64_t parents_stride_b, int B, int L, int Hkv, int d,
+                                    int num_blocks, int block_size, int max_blocks,
+                                    const int64_t* kv_strides, int dtype, const float* rope_cos,
+                                    const float* rope_sin, int rope_max_pos, void* stream) {
+  CIE_CHECK_ARG(parents != nullptr, "cie_rope_append_tree: null pointer");
+  CIE_CHECK_ARG(parents_stride_b >= 0, "cie_rope_append_tree: negative parents stride");
+  CIE_CHECK_ARG(L <= CIE_MAX_TREE, "cie_rope_append_tree: %d nodes, at most %d", L, CIE_MAX_TREE);
+  return rope_append_impl(k_new, v_new, k_pool, v_pool, block_tables, start_pos, parents,
+                          parents_stride_b, B, L, Hkv, d, num_blocks, block_size, max_blocks,
+                          kv_strides, dtype, rope_cos, rope_sin, rope_max_pos, stream);
 }
 
 extern "C" int cie_copy_blocks(void* const* pools, int n_pools, const int32_t* src_blocks,

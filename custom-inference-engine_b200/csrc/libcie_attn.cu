@@ -7,4 +7,5 @@
 #include "paged_noalloc.cu"
 #include "prefill_attn.cu"
 #include "int8_gemm.cu"
+#include "draft_tree.cu"
 #include "peer_barrier.cu"

@@ -25,6 +25,15 @@
 // runs an online softmax (quad shuffles) over its tiles; the 4 warps are
 // merged in shared memory, and split-KV partitions of one sequence by a
 // log-sum-exp merge kernel.
+//
+// Tree variant (TREE = true, cie_tree_attn): the M query rows of a sequence are
+// the nodes of a tree of drafted tokens, in its last M cache slots. Row i sees
+// the kv_len - M history keys and, of the drafted ones, itself and its
+// ancestors: s_ij = scale q_i.k_j for j < kv_len - M or anc[i][j - (kv_len - M)].
+// Each CTA reads the M parent indices once and turns them into one ancestor
+// bitmap per row (RG x ceil(M / 32) words in shared memory), so only the tiles
+// that reach past the history pay for the mask: a 16-bit window per row and
+// tile. Everything before them is the unmasked loop of the decode kernel.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -64,6 +73,9 @@ struct PagedParams {
   int64_t k_sb, k_sh, k_sn;
   int64_t v_sb, v_sh, v_sn;
   int rope_q_pos0;  // dense mode: q row i rotated at rope_q_pos0 + i
+  // tree mode: parent of node i of sequence b at parents[b * par_sb + i]
+  const int32_t* parents;
+  int64_t par_sb;
 };
 
 constexpr int kPagedWarps = 4;
@@ -115,7 +127,12 @@ __host__ __device__ constexpr int paged_smem_bytes() {
          1024;
 }
 
-template <int D, int MT, bool BF16, bool PAGED, bool TMA>
+// Tree mode, behind the shared memory of paged_smem_bytes: M parents, RG depths
+// and RG ancestor bitmaps.
+__host__ __device__ constexpr int tree_words(int M) { return (M + 31) / 32; }
+static int tree_smem_bytes(int M, int rg_rows) { return 4 * (M + rg_rows * (1 + tree_words(M))); }
+
+template <int D, int MT, bool BF16, bool PAGED, bool TMA, bool TREE>
 __global__ void __launch_bounds__(kPagedWarps * 32)
     paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v, const PagedParams p) {
@@ -132,6 +149,10 @@ __global__ void __launch_bounds__(kPagedWarps * 32)
   uint64_t* full_bars = reinterpret_cast<uint64_t*>(qs + RG * D * 2);  // [warps][STAGES]
   volatile int* abort_flag = reinterpret_cast<volatile int*>(full_bars + kPagedWarps * STAGES);
   int* stage_bad = const_cast<int*>(abort_flag) + 4;  // [warps][STAGES]
+  // tree mode (rows of this CTA only)
+  int* s_parent = stage_bad + kPagedWarps * STAGES;  // [M]
+  int* s_depth = s_parent + p.M;                     // [RG]
+  uint32_t* s_anc = reinterpret_cast<uint32_t*>(s_depth + RG);  // [RG][tree_words(M)]
 
   const int split = blockIdx.x;
   const int kvh = blockIdx.y / p.row_groups;
@@ -154,7 +175,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32)
   const int row0 = rg * RG;  // first row of this CTA
   // keys past the last visible key of this CTA's rows are never loaded
   int key_cap = kv_len;
-  if (p.causal) {
+  if (!TREE && p.causal) {
     const int last = min(row0 + RG, R) - 1;
     const int max_m = (row0 / p.M != last / p.M) ? p.M - 1 : last % p.M;
     key_cap = max(0, min(kv_len, kv_len - p.M + max_m + 1));
@@ -293,6 +314,27 @@ __global__ void __launch_bounds__(kPagedWarps * 32)
     if constexpr (!TMA) cp_async_commit();
   }
 
+  if constexpr (TREE) {
+    // ancestor bitmaps of this CTA's rows, while the first K/V tiles are in flight
+    const int32_t* par = p.parents + b * p.par_sb;
+    for (int i = tid; i < p.M; i += blockDim.x) s_parent[i] = tree_parent(par, i);
+    __syncthreads();
+    const int words = tree_words(p.M);
+    for (int r = tid; r < RG; r += blockDim.x) {
+      uint32_t* anc = s_anc + r * words;
+      for (int w = 0; w < words; ++w) anc[w] = 0;
+      int depth = -1;
+      if (row0 + r < R) {
+        for (int j = (row0 + r) % p.M; j >= 0; j = s_parent[j]) {  // indices only fall: ends
+          anc[j >> 5] |= 1u << (j & 31);
+          ++depth;
+        }
+      }
+      s_depth[r] = depth;
+    }
+    __syncthreads();
+  }
+
   // ---- rotated Q tile -> shared memory (16B-chunk swizzle) ----
   {
     using elem_t = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
@@ -311,7 +353,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32)
         const uint4 x1 = *reinterpret_cast<const uint4*>(src + pc * 8);
         const uint4 x2 = *reinterpret_cast<const uint4*>(src + HALF + pc * 8);
         if (p.cos != nullptr) {
-          int pos = q_pos_base + m;
+          int pos = q_pos_base + (TREE ? s_depth[r] : m);
           if (pos < 0 || pos >= p.rope_max_pos) {
             raise_status(CIE_DEV_BAD_POSITION);
             pos = pos < 0 ? 0 : p.rope_max_pos - 1;
@@ -372,6 +414,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32)
       lim[mt][hf] = p.causal ? (kv_len - p.M + m) : (kv_len - 1);
     }
   const int lim_min = p.causal ? (kv_len - p.M) : (kv_len - 1);
+  const int hist = kv_len - p.M;  // tree mode: keys before the drafted ones (< 0: slots missing)
 
   for (int it = 0; it < my_tiles; ++it) {
     {
@@ -446,7 +489,30 @@ __global__ void __launch_bounds__(kPagedWarps * 32)
     }
 
     // online softmax (log2 domain); O is rescaled only when a row's max grew by > 2^8
-    const bool need_mask = (t0 + kTileTok - 1) > lim_min;
+    const bool need_mask = (t0 + kTileTok - 1) > (TREE ? hist - 1 : lim_min);
+    // tree mode: bit c of a row's window = key t0 + c is visible to it
+    uint32_t win[TREE ? MT : 1][2];
+    if constexpr (TREE) {
+      if (need_mask) {
+        const int words = tree_words(p.M);
+        const int j0 = t0 - hist;  // node of the tile's first key; >= -15 here
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            const uint32_t* anc = s_anc + (mt * 16 + g + 8 * hf) * words;
+            uint32_t w;
+            if (j0 < 0) {
+              w = (anc[0] << -j0) | ((1u << -j0) - 1u);
+            } else {
+              const int i = j0 >> 5, sh = j0 & 31;
+              w = anc[i] >> sh;
+              if (sh > 32 - kTileTok && i + 1 < words) w |= anc[i + 1] << (32 - sh);
+            }
+            win[mt][hf] = w;
+          }
+      }
+    }
     // fp16: P = p_hi + p_lo, both fp16, so the PV product sees P to about 2^-22
     // relative instead of one rounding's 2^-12 and the output matches the fp32
     // reference to within one fp16 rounding (the reference's own fp16 kernel
@@ -469,8 +535,12 @@ __global__ void __launch_bounds__(kPagedWarps * 32)
           for (int e = 0; e < 2; ++e) {
             float x = s[mt][nt][2 * hf + e] * p.scale_log2;
             if (need_mask) {
-              const int tok = t0 + nt * 8 + 2 * t4 + e;
-              if (tok > lim[mt][hf]) x = -INFINITY;
+              if constexpr (TREE) {
+                if (!((win[mt][hf] >> (nt * 8 + 2 * t4 + e)) & 1u)) x = -INFINITY;
+              } else {
+                const int tok = t0 + nt * 8 + 2 * t4 + e;
+                if (tok > lim[mt][hf]) x = -INFINITY;
+              }
             }
             v[nt * 2 + e] = x;
           }
@@ -513,6 +583,55 @@ __global__ void __launch_bounds__(kPagedWarps * 32)
           o_acc[mt][nt][2] *= alpha[mt][1];
           o_acc[mt][nt][3] *= alpha[mt][1];
         }
+    }
+
+    if constexpr (TREE) {
+      // A node's V row that holds NaN or infinity must not reach the rows that do
+      // not see it, and 0 x NaN in the MMA below would: such rows (none, as a rule)
+      // are added here for the rows that see them and then zeroed in the tile.
+      if (need_mask) {
+        uint32_t bad = 0;  // lane's share: 16-bit elements whose exponent is all ones
+        for (int q = lane; q < kTileTok * KC; q += 32) {
+          const uint4 x = *reinterpret_cast<const uint4*>(vs + kv_off<D>(q / KC, q % KC));
+          constexpr uint32_t kExp = BF16 ? 0x7f80u : 0x7c00u;
+          const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+          bool nf = false;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            nf |= (u[e] & kExp) == kExp || (u[e] & (kExp << 16)) == (kExp << 16);
+          if (nf) bad |= 1u << (q / KC);
+        }
+        bad = __reduce_or_sync(0xffffffffu, bad);
+        for (uint32_t left = bad; left != 0; left &= left - 1) {
+          const int j = __ffs(left) - 1;
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+              // P of (row, key j) sits in lane (row's quad) + (j % 8) / 2
+              const int src = (lane & ~3) | ((j & 7) >> 1);
+              const uint32_t pw = __shfl_sync(0xffffffffu, j < 8 ? pa[mt][hf] : pa[mt][2 + hf], src);
+              const float2 pf = unpack2<BF16>(pw);
+              const float pj = (j & 1) ? pf.y : pf.x;
+              if ((win[mt][hf] >> j) & 1u) {
+#pragma unroll
+                for (int nt = 0; nt < D / 8; ++nt) {
+                  const uint32_t vw = *reinterpret_cast<const uint32_t*>(vs + kv_off<D>(j, nt) + t4 * 4);
+                  const float2 vf = unpack2<BF16>(vw);
+                  o_acc[mt][nt][2 * hf] += pj * vf.x;
+                  o_acc[mt][nt][2 * hf + 1] += pj * vf.y;
+                }
+              }
+            }
+        }
+        if (bad != 0) {
+          __syncwarp();
+          for (int q = lane; q < kTileTok * KC; q += 32)
+            if ((bad >> (q / KC)) & 1u)
+              *reinterpret_cast<uint4*>(vs + kv_off<D>(q / KC, q % KC)) = make_uint4(0, 0, 0, 0);
+          __syncwarp();
+        }
+      }
     }
 
     // O += P V
@@ -601,8 +720,10 @@ __global__ void __launch_bounds__(kPagedWarps * 32)
       else o[b * p.o_sb + h * p.o_sh + m * p.o_sm + d] = __float2half_rn(out);
     } else {
       const int64_t base = (static_cast<int64_t>(unit) * p.max_splits + split) * RG;
-      p.part_o[(base + r) * D + d] = l > 0.f ? acc / l : 0.f;
-      if (d == 0) p.part_lse[base + r] = l > 0.f ? mu + __log2f(l) : -INFINITY;
+      // tree mode: a NaN sum (l == l false) goes on to the merge as a NaN weight
+      const bool live = TREE ? !(l <= 0.f) : l > 0.f;
+      p.part_o[(base + r) * D + d] = live ? acc / l : 0.f;
+      if (d == 0) p.part_lse[base + r] = live ? mu + __log2f(l) : -INFINITY;
     }
   }
 }
@@ -760,11 +881,11 @@ static bool make_kv_map(CUtensorMap* map, const void* base, int d, const cuuint6
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D, int MT, bool BF16, bool PAGED, bool TMA>
+template <int D, int MT, bool BF16, bool PAGED, bool TMA, bool TREE>
 static int launch_mma_t(const CUtensorMap& mk, const CUtensorMap& mv, const PagedParams& prm,
                         cudaStream_t st) {
-  constexpr int smem = paged_smem_bytes<D, MT>();
-  auto kern = paged_attn_kernel<D, MT, BF16, PAGED, TMA>;
+  const int smem = paged_smem_bytes<D, MT>() + (TREE ? tree_smem_bytes(prm.M, 16 * MT) : 0);
+  auto kern = paged_attn_kernel<D, MT, BF16, PAGED, TMA, TREE>;
   cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   dim3 grid(prm.max_splits, prm.Hkv * prm.row_groups, prm.B);
   kern<<<grid, kPagedWarps * 32, smem, st>>>(mk, mv, prm);
@@ -779,7 +900,7 @@ static int launch_mma_t(const CUtensorMap& mk, const CUtensorMap& mv, const Page
   return CIE_OK;
 }
 
-template <int D, int MT, bool BF16, bool PAGED>
+template <int D, int MT, bool BF16, bool PAGED, bool TREE>
 static int launch_mma(const PagedParams& prm, cudaStream_t st) {
   // TMA feeds need a 16-token tile inside one block (paged) and 16-byte
   // aligned rows; otherwise the cp.async path serves the call.
@@ -810,39 +931,39 @@ static int launch_mma(const PagedParams& prm, cudaStream_t st) {
     tma = ok_strides && make_kv_map(&mk, prm.k_pool, D, dims, ks, box, bf16) &&
           make_kv_map(&mv, prm.v_pool, D, dims, vs, box, bf16);
   }
-  if (tma) return launch_mma_t<D, MT, BF16, PAGED, true>(mk, mv, prm, st);
-  return launch_mma_t<D, MT, BF16, PAGED, false>(mk, mv, prm, st);
+  if (tma) return launch_mma_t<D, MT, BF16, PAGED, true, TREE>(mk, mv, prm, st);
+  return launch_mma_t<D, MT, BF16, PAGED, false, TREE>(mk, mv, prm, st);
 }
 
-template <int D, bool BF16, bool PAGED>
+template <int D, bool BF16, bool PAGED, bool TREE>
 static int dispatch_mt(const PagedParams& prm, int mt, cudaStream_t st) {
   if constexpr (D >= 256) {
-    return launch_mma<D, 1, BF16, PAGED>(prm, st);
+    return launch_mma<D, 1, BF16, PAGED, TREE>(prm, st);
   } else if constexpr (D == 128) {
-    return mt == 1 ? launch_mma<D, 1, BF16, PAGED>(prm, st)
-                   : launch_mma<D, 2, BF16, PAGED>(prm, st);
+    return mt == 1 ? launch_mma<D, 1, BF16, PAGED, TREE>(prm, st)
+                   : launch_mma<D, 2, BF16, PAGED, TREE>(prm, st);
   } else {
     switch (mt) {
-      case 1: return launch_mma<D, 1, BF16, PAGED>(prm, st);
-      case 2: return launch_mma<D, 2, BF16, PAGED>(prm, st);
-      default: return launch_mma<D, 4, BF16, PAGED>(prm, st);
+      case 1: return launch_mma<D, 1, BF16, PAGED, TREE>(prm, st);
+      case 2: return launch_mma<D, 2, BF16, PAGED, TREE>(prm, st);
+      default: return launch_mma<D, 4, BF16, PAGED, TREE>(prm, st);
     }
   }
 }
 
-template <bool PAGED>
+template <bool PAGED, bool TREE = false>
 static int dispatch_d(const PagedParams& prm, int d, int mt, bool bf16, cudaStream_t st) {
   switch (d) {
-    case 16: return bf16 ? dispatch_mt<16, true, PAGED>(prm, mt, st)
-                         : dispatch_mt<16, false, PAGED>(prm, mt, st);
-    case 32: return bf16 ? dispatch_mt<32, true, PAGED>(prm, mt, st)
-                         : dispatch_mt<32, false, PAGED>(prm, mt, st);
-    case 64: return bf16 ? dispatch_mt<64, true, PAGED>(prm, mt, st)
-                         : dispatch_mt<64, false, PAGED>(prm, mt, st);
-    case 128: return bf16 ? dispatch_mt<128, true, PAGED>(prm, mt, st)
-                          : dispatch_mt<128, false, PAGED>(prm, mt, st);
-    case 256: return bf16 ? dispatch_mt<256, true, PAGED>(prm, mt, st)
-                          : dispatch_mt<256, false, PAGED>(prm, mt, st);
+    case 16: return bf16 ? dispatch_mt<16, true, PAGED, TREE>(prm, mt, st)
+                         : dispatch_mt<16, false, PAGED, TREE>(prm, mt, st);
+    case 32: return bf16 ? dispatch_mt<32, true, PAGED, TREE>(prm, mt, st)
+                         : dispatch_mt<32, false, PAGED, TREE>(prm, mt, st);
+    case 64: return bf16 ? dispatch_mt<64, true, PAGED, TREE>(prm, mt, st)
+                         : dispatch_mt<64, false, PAGED, TREE>(prm, mt, st);
+    case 128: return bf16 ? dispatch_mt<128, true, PAGED, TREE>(prm, mt, st)
+                          : dispatch_mt<128, false, PAGED, TREE>(prm, mt, st);
+    case 256: return bf16 ? dispatch_mt<256, true, PAGED, TREE>(prm, mt, st)
+                          : dispatch_mt<256, false, PAGED, TREE>(prm, mt, st);
     default:
       set_error("attention: head_dim %d unsupported", d);
       return CIE_ERR_UNSUPPORTED;
@@ -1005,4 +1126,75 @@ extern "C" int cie_paged_attn(const void* q, const void* k_pool, const void* v_p
   prm.bs_log2 = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1;
   return dispatch_d<true>(prm, d, pl.mt, dtype == CIE_DTYPE_BF16,
                           reinterpret_cast<cudaStream_t>(stream));
+}
+
+// ------------------------------------------------------------------ tree of drafts
+extern "C" size_t cie_tree_attn_workspace(int B, int Hq, int Hkv, int T, int d, int block_size,
+                                          int max_blocks, int split_tokens) {
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || T <= 0 || Hq % Hkv != 0 || !mma_head_dim_ok(d) ||
+      block_size <= 0 || max_blocks < 0)
+    return 0;
+  return make_plan(B, Hq, Hkv, T, d, max_blocks * block_size, split_tokens).workspace();
+}
+
+extern "C" int cie_tree_attn(const void* q, const void* k_pool, const void* v_pool,
+                             const int32_t* block_tables, const int32_t* kv_lens,
+                             const int32_t* parents, int64_t parents_stride_b, void* o, int B,
+                             int Hq, int Hkv, int T, int d, int num_blocks, int block_size,
+                             int max_blocks, const int64_t* q_strides, const int64_t* o_strides,
+                             float scale, int dtype, const float* rope_cos, const float* rope_sin,
+                             int rope_max_pos, int split_tokens, void* workspace,
+                             size_t workspace_bytes, void* stream) {
+  CIE_CHECK_ARG(q && k_pool && v_pool && block_tables && kv_lens && parents && o,
+                "cie_tree_attn: null tensor pointer");
+  CIE_CHECK_ARG(B >= 0 && Hq > 0 && Hkv > 0 && T >= 0, "cie_tree_attn: bad shape");
+  CIE_CHECK_ARG(Hq % Hkv == 0, "cie_tree_attn: Hq (%d) must be a multiple of Hkv (%d)", Hq, Hkv);
+  CIE_CHECK_ARG(T <= CIE_MAX_TREE, "cie_tree_attn: %d nodes, at most %d", T, CIE_MAX_TREE);
+  CIE_CHECK_ARG(parents_stride_b >= 0, "cie_tree_attn: negative parents stride");
+  CIE_CHECK_ARG(dtype == CIE_DTYPE_BF16 || dtype == CIE_DTYPE_FP16, "cie_tree_attn: bad dtype %d",
+                dtype);
+  CIE_CHECK_ARG(num_blocks > 0 && block_size > 0 && max_blocks > 0,
+                "cie_tree_attn: bad pool geometry");
+  CIE_CHECK_ARG(static_cast<int64_t>(max_blocks) * block_size < (int64_t(1) << 31) - 4096,
+                "cie_tree_attn: max_blocks * block_size too large");
+  CIE_CHECK_ARG(q_strides && o_strides, "cie_tree_attn: null strides");
+  CIE_CHECK_ARG(aligned16(q) && aligned16(k_pool) && aligned16(v_pool),
+                "cie_tree_attn: q/k_pool/v_pool must be 16-byte aligned");
+  CIE_CHECK_ARG(q_strides[0] % 8 == 0 && q_strides[1] % 8 == 0 && q_strides[2] % 8 == 0,
+                "cie_tree_attn: q strides must be multiples of 8 elements");
+  CIE_CHECK_ARG(split_tokens == 0 || (split_tokens > 0 && split_tokens % 16 == 0),
+                "cie_tree_attn: split_tokens must be 0 or a positive multiple of 16");
+  CIE_CHECK_ARG((rope_cos == nullptr) == (rope_sin == nullptr),
+                "cie_tree_attn: rope_cos and rope_sin must both be given or both NULL");
+  CIE_CHECK_ARG(rope_cos == nullptr || rope_max_pos > 0, "cie_tree_attn: rope_max_pos <= 0");
+  if (!mma_head_dim_ok(d)) {
+    set_error("cie_tree_attn: head_dim %d unsupported (16, 32, 64, 128 or 256)", d);
+    return CIE_ERR_UNSUPPORTED;
+  }
+  if (B == 0 || T == 0) return CIE_OK;
+  const MmaPlan pl = make_plan(B, Hq, Hkv, T, d, max_blocks * block_size, split_tokens);
+  if (pl.workspace() > 0 && (workspace == nullptr || workspace_bytes < pl.workspace())) {
+    set_error("cie_tree_attn: workspace of %zu bytes required, got %zu", pl.workspace(),
+              workspace_bytes);
+    return CIE_ERR_WORKSPACE;
+  }
+  if (B > 65535 || static_cast<int64_t>(Hkv) * pl.row_groups > 65535) {
+    set_error("cie_tree_attn: grid too large (B=%d, Hkv*row_groups=%d)", B, Hkv * pl.row_groups);
+    return CIE_ERR_UNSUPPORTED;
+  }
+  PagedParams prm{};
+  fill_common(prm, pl, q, o, B, Hq, Hkv, T, q_strides, o_strides, scale, 0, rope_cos, rope_sin,
+              rope_max_pos, workspace);
+  prm.k_pool = k_pool;
+  prm.v_pool = v_pool;
+  prm.block_tables = block_tables;
+  prm.kv_lens = kv_lens;
+  prm.num_blocks = num_blocks;
+  prm.block_size = block_size;
+  prm.max_blocks = max_blocks;
+  prm.bs_log2 = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1;
+  prm.parents = parents;
+  prm.par_sb = parents_stride_b;
+  return dispatch_d<true, true>(prm, d, pl.mt, dtype == CIE_DTYPE_BF16,
+                                reinterpret_cast<cudaStream_t>(stream));
 }

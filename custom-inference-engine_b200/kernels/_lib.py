@@ -25,16 +25,22 @@ CIE_ERR_DEVICE = -5
 
 CIE_DTYPE_BF16 = 0
 CIE_DTYPE_FP16 = 1
+CIE_DTYPE_FP32 = 2
+
+CIE_MAX_TREE = 1024
 
 CIE_DEV_BAD_BLOCK_ID = 0x1
 CIE_DEV_TIMEOUT = 0x2
 CIE_DEV_BAD_POSITION = 0x4
+CIE_DEV_BAD_TREE = 0x8
+CIE_DEV_BAD_PROBS = 0x10
 
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _f = ctypes.c_float
 _sz = ctypes.c_size_t
 _i64p = ctypes.POINTER(ctypes.c_int64)
+_i64 = ctypes.c_int64
 
 # name -> (restype, argtypes); must match include/cie_attn.h
 SIGNATURES: dict[str, tuple] = {
@@ -53,6 +59,15 @@ SIGNATURES: dict[str, tuple] = {
     "cie_gather_kv": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp]),
     "cie_rope_append": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i64p,
                              _i, _vp, _vp, _i, _vp]),
+    "cie_rope_append_tree": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _i, _i, _i,
+                                  _i, _i64p, _i, _vp, _vp, _i, _vp]),
+    "cie_tree_attn": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i, _i, _i, _i, _i, _i, _i, _i,
+                           _i64p, _i64p, _f, _i, _vp, _vp, _i, _i, _vp, _sz, _vp]),
+    "cie_tree_attn_workspace": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i]),
+    "cie_verify_drafts": (_i, [_vp, _i64, _i, _vp, _i64, _vp, _i64p, _vp, _i64p, _i, _vp, _i64, _i,
+                               _i, _i, _i, _vp, _vp, _vp, _vp]),
+    "cie_keep_path": (_i, [ctypes.POINTER(_vp), _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i,
+                           _sz, _vp]),
     "cie_copy_blocks": (_i, [ctypes.POINTER(_vp), _i, _vp, _vp, _i, _i, _sz, _vp]),
     "cie_rope": (_i, [_vp, _vp, _i, _i, _i, _i, _i64p, _i64p, _i, _i, _vp, _vp, _i, _vp]),
     "cie_int8_matmul": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, ctypes.c_int64,

@@ -302,12 +302,16 @@ def rope_append(
     block_tables: torch.Tensor,
     start_pos: torch.Tensor,
     rope: tuple[torch.Tensor, torch.Tensor] | None = None,
+    parents: torch.Tensor | None = None,
 ) -> None:
     """Write k_new/v_new (B, L, Hkv, D) into the pools at positions start_pos[b] + i.
 
     K rows are rotated at their positions when ``rope`` is given (the cache stores
     rotated K, as the reference does at engine/model/block.py:53-64). Blocks must
-    already be assigned in ``block_tables``.
+    already be assigned in ``block_tables``. ``parents``: int32 (L,) or (B, L), the
+    tree of drafted tokens whose nodes the L rows are (see ``kernels.draft_tree``):
+    row i still goes to slot start_pos[b] + i, but K is rotated at position
+    start_pos[b] + depth of node i.
     """
     if not k_new.is_cuda:
         raise RuntimeError("rope_append requires CUDA tensors")
@@ -328,6 +332,18 @@ def rope_append(
         k_new = k_new.contiguous()
         v_new = v_new.contiguous()
     cos, sin, max_pos = _rope_tables(rope, k_new.device)
+    if parents is not None:
+        from kernels.draft_tree import _parents
+
+        parents, par_sb = _parents(parents, B, L, k_new.device, "rope_append")
+        with torch.cuda.device(k_new.device):
+            rc = lib.cie_rope_append_tree(
+                _vp(k_new), _vp(v_new), _vp(k_pool), _vp(v_pool), _vp(block_tables.contiguous()),
+                _vp(start_pos.contiguous()), _vp(parents), par_sb, B, L, Hkv, D, nb, bs,
+                block_tables.shape[1], _lib.strides3(k_new.stride()[:3]), _DTYPES[k_new.dtype],
+                _vp(cos), _vp(sin), max_pos, _stream(k_new))
+        _lib.check(rc, "rope_append")
+        return
     rc = lib.cie_rope_append(
         _vp(k_new), _vp(v_new), _vp(k_pool), _vp(v_pool), _vp(block_tables.contiguous()),
         _vp(start_pos.contiguous()), B, L, Hkv, D, nb, bs, block_tables.shape[1],

@@ -38,12 +38,17 @@ enum cie_status {
   CIE_ERR_DEVICE = -5        /* device-side status word is non-zero            */
 };
 
-enum cie_dtype { CIE_DTYPE_BF16 = 0, CIE_DTYPE_FP16 = 1 };
+/* FP32: cie_verify_drafts only */
+enum cie_dtype { CIE_DTYPE_BF16 = 0, CIE_DTYPE_FP16 = 1, CIE_DTYPE_FP32 = 2 };
+
+#define CIE_MAX_TREE 1024 /* nodes of a tree of drafted tokens */
 
 /* Device status bits (cie_device_status). */
 #define CIE_DEV_BAD_BLOCK_ID 0x1  /* a block-table entry was < 0 or >= num_blocks */
 #define CIE_DEV_TIMEOUT 0x2       /* a bounded pipeline wait expired               */
 #define CIE_DEV_BAD_POSITION 0x4  /* a RoPE position fell outside the cos/sin table */
+#define CIE_DEV_BAD_TREE 0x8      /* a parent, token or path entry that no tree has     */
+#define CIE_DEV_BAD_PROBS 0x10    /* a row of probabilities without a finite, positive sum */
 
 /*
  * Dense causal / non-causal grouped-query attention (prefill).
@@ -223,6 +228,107 @@ int cie_rope_append(const void* k_new, const void* v_new, void* k_pool,
                     const int64_t* kv_strides, int dtype,
                     const float* rope_cos, const float* rope_sin,
                     int rope_max_pos, void* stream);
+
+/*
+ * cie_rope_append for the nodes of a tree of drafted tokens: row i of sequence
+ * b goes to slot start_pos[b] + i as above, but its K is rotated at position
+ * start_pos[b] + depth(i), depth counting i's ancestors in the tree that
+ * parents (B or 1, L) int32 gives (parent of node i below i, -1 none; row
+ * stride parents_stride_b, 0 = one tree for all). L <= CIE_MAX_TREE. A parent
+ * that is no index below its node sets CIE_DEV_BAD_TREE and counts as none.
+ */
+int cie_rope_append_tree(const void* k_new, const void* v_new, void* k_pool,
+                         void* v_pool, const int32_t* block_tables,
+                         const int32_t* start_pos, const int32_t* parents,
+                         int64_t parents_stride_b, int B, int L, int Hkv, int d,
+                         int num_blocks, int block_size, int max_blocks,
+                         const int64_t* kv_strides, int dtype,
+                         const float* rope_cos, const float* rope_sin,
+                         int rope_max_pos, void* stream);
+
+/*
+ * Attention of a tree of T drafted tokens a sequence over its paged history.
+ * As cie_paged_attn (same pools, tables, strides, workspace and split), but the
+ * T query rows are the nodes of a tree that occupies the last T of the
+ * kv_lens[b] slots: node i sits in slot kv_lens[b] - T + i and sees the
+ * kv_lens[b] - T keys of the history, itself and its ancestors:
+ *   parents: int32 (B or 1, T), row stride parents_stride_b (0 = one tree for
+ *            the batch); parents[i] < i is node i's parent, -1 none.
+ * A chain (parents[i] = i - 1) is cie_paged_attn with causal = 1. With RoPE
+ * tables row i of q is rotated at kv_lens[b] - T + depth(i). NaN or infinity in
+ * the K or V row of a node reaches only the rows that see it. A sequence with
+ * kv_lens[b] = 0 gives zeros; a node whose slot would lie before the first
+ * (0 < kv_lens[b] < T) sees no key and gives NaN. Bad parents: as above.
+ * T <= CIE_MAX_TREE.
+ */
+int cie_tree_attn(const void* q, const void* k_pool, const void* v_pool,
+                  const int32_t* block_tables, const int32_t* kv_lens,
+                  const int32_t* parents, int64_t parents_stride_b, void* o,
+                  int B, int Hq, int Hkv, int T, int d, int num_blocks,
+                  int block_size, int max_blocks, const int64_t* q_strides,
+                  const int64_t* o_strides, float scale, int dtype,
+                  const float* rope_cos, const float* rope_sin,
+                  int rope_max_pos, int split_tokens, void* workspace,
+                  size_t workspace_bytes, void* stream);
+
+/* Bytes of workspace cie_tree_attn needs for these arguments. */
+size_t cie_tree_attn_workspace(int B, int Hq, int Hkv, int T, int d,
+                               int block_size, int max_blocks, int split_tokens);
+
+/*
+ * Which nodes of a tree of drafted tokens are kept, and the token behind them:
+ * speculative sampling from given uniform numbers, or greedily. The reference
+ * verifies one greedy chain on the host (engine/decode/speculative.py:88-123).
+ *   tokens:   (B, T) int32, or int64 when tokens_64bit; node 0, the root, is the
+ *             last token that was kept before
+ *   parents:  as above; node 0 is the root
+ *   target:   (B, T, V) in dtype (any cie_dtype): row i is the target model's
+ *             distribution after node i. strides: B and T dims, elements.
+ *   draft:    NULL, or (B, draft_rows, V): row i is the distribution that the
+ *             children of node i were drawn from, independently of one another.
+ *             Nodes from draft_rows on are leaves. NULL: the children were
+ *             chosen, not drawn (all the mass of the draft is on the child).
+ *   uniforms: (B, T) fp32 in [0, 1): entry i decides node i, entry 0 the last
+ *             token. NULL: greedy; target may then hold logits and draft is NULL.
+ * At a node with r = target row and m = 1, children are tested in index order:
+ * kept if u draft(x) m < r(x); else r = max(r - m draft, 0), m = sum of r (draft
+ * NULL: draft(x) = 1; r(x) leaves m and is set to 0). No child kept: the last
+ * token is the first v with cumsum(r)[v] > uniforms[b, 0] * sum(r); if r has no
+ * mass, of the target row itself. Greedy: the child that drafted the row's
+ * largest entry (ties: the lowest index) is kept; without one that entry is the
+ * last token. All of this in 64 bits.
+ *   path:       int32 (B, T): the kept nodes, root first, then -1
+ *   n:          int32 (B,): their number, at least 1
+ *   out_tokens: (B, T) in tokens' type: the tokens of path[1..n-1], the last
+ *               token, then -1
+ * A target row without a finite positive sum gives the last token -1 and sets
+ * CIE_DEV_BAD_PROBS; a drafted token outside [0, V) is never kept and sets
+ * CIE_DEV_BAD_TREE. Outputs contiguous. T <= CIE_MAX_TREE, V <= 2^23.
+ */
+int cie_verify_drafts(const void* tokens, int64_t tokens_stride_b,
+                      int tokens_64bit, const int32_t* parents,
+                      int64_t parents_stride_b, const void* target,
+                      const int64_t* target_strides, const void* draft,
+                      const int64_t* draft_strides, int draft_rows,
+                      const float* uniforms, int64_t uniforms_stride_b, int B,
+                      int T, int V, int dtype, void* out_tokens, int32_t* path,
+                      int32_t* n, void* stream);
+
+/*
+ * Moves the kept nodes' K and V rows behind the history, in every pool, in
+ * place: for 1 <= i < n[b]
+ *   pool[slot base + i] = pool[slot base + path[b, i]],  base = kv_lens[b] - T
+ * and new_lens[b] = max(0, base + n[b]) (new_lens may be NULL). pools: host
+ * array of n_pools device pointers, each to num_blocks * block_size rows of
+ * row_bytes bytes (a multiple of 16). path rises, as cie_verify_drafts gives it;
+ * an entry below its index or beyond T is skipped and sets CIE_DEV_BAD_TREE. One
+ * launch per 256 pools. Two sequences must not share a block that is written.
+ */
+int cie_keep_path(void* const* pools, int n_pools, const int32_t* block_tables,
+                  const int32_t* kv_lens, const int32_t* path, const int32_t* n,
+                  int32_t* new_lens, int B, int T, int num_blocks,
+                  int block_size, int max_blocks, size_t row_bytes,
+                  void* stream);
 
 /*
  * Whole-block copies inside paged pools, the data movement of
