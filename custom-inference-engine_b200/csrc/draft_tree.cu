@@ -42,8 +42,10 @@ namespace cg = cooperative_groups;
 // (entries, gathers, row, drawn segment).
 constexpr int kVfThreads = 512;
 constexpr int kVfWarps = kVfThreads / 32;
-constexpr int kSeg = 1024;        // elements of a row summed by one warp at a time
+constexpr int kSeg = 512;         // elements of a row summed by one warp at a time; one per
+                                  // thread when the drawn token is looked for in it
 constexpr int kVfMaxCluster = 8;  // portable cluster size
+static_assert(kSeg == kVfThreads, "the search gives every thread one element");
 
 struct VerifyParams {
   const void* tokens;  // (B, T) int32 or int64
@@ -116,7 +118,9 @@ __global__ void __launch_bounds__(kVfThreads) verify_kernel(const VerifyParams p
   __shared__ double s_cum[kVfMaxCluster + 1];                   // shares of the CTAs before each, and all
   __shared__ unsigned long long s_warp[kVfWarps];
   __shared__ double s_c;                                        // r = max(p - s_c q, 0)
+  __shared__ double s_before;                                 // sum before the drawn segment
   __shared__ int s_cur, s_len, s_ngone, s_done, s_best;
+  __shared__ int s_first, s_last, s_which;                      // the search for the last token
 
   cg::cluster_group cluster = cg::this_cluster();
   const int CL = static_cast<int>(cluster.num_blocks());
@@ -273,25 +277,27 @@ __global__ void __launch_bounds__(kVfThreads) verify_kernel(const VerifyParams p
           if (gone || e0 + kSeg > p.V) {  // an edge or an excluded token: one element at a time
             for (int64_t at = e0 + lane; at < e0 + kSeg && at < p.V; at += 32)
               sum += left_at(pr, qr, c, at, gone);
-          } else if (qr != nullptr) {
-#pragma unroll 4
-            for (int j = 0; j < kSeg / (32 * VEC); ++j) {
-              const int64_t at = e0 + (j * 32 + lane) * VEC;
-              float x[VEC], y[VEC];
-              load_row<T, VEC>(pr + at, x);
-              load_row<T, VEC>(qr + at, y);
-#pragma unroll
-              for (int e = 0; e < VEC; ++e) sum += residual(x[e], y[e], c);
-            }
           } else {
-#pragma unroll 8
-            for (int j = 0; j < kSeg / (32 * VEC); ++j) {
-              const int64_t at = e0 + (j * 32 + lane) * VEC;
-              float x[VEC];
-              load_row<T, VEC>(pr + at, x);
+            // all of the lane's loads first, then four chains of additions
+            constexpr int kStep = kSeg / (32 * VEC) < 8 ? kSeg / (32 * VEC) : 8;
+            double acc[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
-              for (int e = 0; e < VEC; ++e) sum += residual(x[e]);
+            for (int j0 = 0; j0 < kSeg / (32 * VEC); j0 += kStep) {
+              float x[kStep][VEC], y[kStep][VEC];
+#pragma unroll
+              for (int j = 0; j < kStep; ++j) {
+                const int64_t at = e0 + ((j0 + j) * 32 + lane) * VEC;
+                load_row<T, VEC>(pr + at, x[j]);
+                if (qr != nullptr) load_row<T, VEC>(qr + at, y[j]);
+              }
+#pragma unroll
+              for (int j = 0; j < kStep; ++j)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e)
+                  acc[(j * VEC + e) & 3] +=
+                      qr != nullptr ? residual(x[j][e], y[j][e], c) : residual(x[j][e]);
             }
+            sum = (acc[0] + acc[1]) + (acc[2] + acc[3]);
           }
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -300,8 +306,11 @@ __global__ void __launch_bounds__(kVfThreads) verify_kernel(const VerifyParams p
       }
       __syncthreads();
       double mine = 0.0;
-      if (tid == 0)
-        for (int s = 0; s < p.segs; ++s) mine += s_seg[s];
+      if (warp == 0) {
+        for (int s = lane; s < p.segs; s += 32) mine += s_seg[s];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+      }
       const unsigned long long got =
           exchange(static_cast<unsigned long long>(__double_as_longlong(mine)));
       if (warp == 0) {
@@ -398,56 +407,68 @@ __global__ void __launch_bounds__(kVfThreads) verify_kernel(const VerifyParams p
         raise_status(CIE_DEV_BAD_PROBS);
         put(-1);
       }
-    } else if (warp == 0) {
+    } else {
       const double u0 = fmin(static_cast<double>(s_u[0]), 1.0 - 0x1p-24);
       const double want = (u0 > 0.0 ? u0 : 0.0) * total;
       int owner = CL - 1;
       for (int r = CL - 1; r >= 0; --r)
         if (s_cum[r + 1] > want) owner = r;
       if (owner == rank) {
-        // the segment, then the element, where the running sum passes `want`
-        double cum = s_cum[rank];
-        int seg = -1;
-        double before = cum;
-        for (int s = 0; s < p.segs; ++s) {
-          if (s_seg[s] > 0.0) {
-            seg = s;  // also the answer if rounding leaves the sum just short
-            before = cum;
-          }
-          cum += s_seg[s];
-          if (cum > want) break;
-        }
-        const T* pr = prow + s_cur * p.p_st;
-        const T* qr = s_c > 0.0 ? qrow + s_cur * p.q_st : nullptr;
-        const int64_t e0 = static_cast<int64_t>(seg0 + seg) * kSeg;
-        const bool gone = gone_in(e0);
-        int64_t found = -1, last = -1;
-        constexpr int kPer = kSeg / 32;  // elements of a lane, one coalesced line at a time
-        for (int j0 = 0; j0 < kPer && found < 0; j0 += 8) {
-          double r[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int64_t e = e0 + (j0 + j) * 32 + lane;
-            r[j] = e < p.V ? left_at(pr, qr, s_c, e, gone) : 0.0;
-          }
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            if (found >= 0) continue;
-            double inc = r[j];
+        // warp 0: the segment where the running sum passes `want` (the last one with
+        // mass if rounding leaves it just short), and the sum before it
+        if (warp == 0) {
+          double before = s_cum[rank];
+          int seg = -1;
+          double seg_before = before;
+          for (int s0 = 0; s0 < p.segs; s0 += 32) {
+            const double mass = s0 + lane < p.segs ? s_seg[s0 + lane] : 0.0;
+            double inc = mass;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
               const double y = __shfl_up_sync(0xffffffffu, inc, o);
               if (lane >= o) inc += y;
             }
-            const int64_t e = e0 + (j0 + j) * 32;
-            const uint32_t over = __ballot_sync(0xffffffffu, r[j] > 0.0 && before + inc > want);
-            const uint32_t some = __ballot_sync(0xffffffffu, r[j] > 0.0);
-            if (over) found = e + __ffs(over) - 1;
-            if (some) last = e + 31 - __clz(some);
+            const uint32_t some = __ballot_sync(0xffffffffu, mass > 0.0);
+            const uint32_t over = __ballot_sync(0xffffffffu, mass > 0.0 && before + inc > want);
+            if (some) {
+              const int at = over ? __ffs(over) - 1 : 31 - __clz(some);
+              seg = s0 + at;
+              seg_before = before + __shfl_sync(0xffffffffu, inc - mass, at);
+            }
+            if (over) break;
             before += __shfl_sync(0xffffffffu, inc, 31);
           }
+          if (lane == 0) {
+            s_which = seg;
+            s_before = seg_before;
+            s_first = kSeg;
+            s_last = -1;
+          }
         }
-        if (lane == 0) put(found >= 0 ? found : last);
+        __syncthreads();
+        // every thread one element of it: the first where the running sum passes
+        const T* pr = prow + s_cur * p.p_st;
+        const T* qr = s_c > 0.0 ? qrow + s_cur * p.q_st : nullptr;
+        const int64_t e0 = static_cast<int64_t>(seg0 + s_which) * kSeg;
+        const bool gone = gone_in(e0);
+        const double r = e0 + tid < p.V ? left_at(pr, qr, s_c, e0 + tid, gone) : 0.0;
+        double inc = r;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double y = __shfl_up_sync(0xffffffffu, inc, o);
+          if (lane >= o) inc += y;
+        }
+        if (lane == 31) s_warp[warp] = static_cast<unsigned long long>(__double_as_longlong(inc));
+        __syncthreads();
+        double before = s_before;
+        for (int w = 0; w < warp; ++w)
+          before += __longlong_as_double(static_cast<long long>(s_warp[w]));
+        if (r > 0.0) {
+          atomicMax(&s_last, tid);
+          if (before + inc > want) atomicMin(&s_first, tid);
+        }
+        __syncthreads();
+        if (tid == 0) put(e0 + (s_first < kSeg ? s_first : s_last));
       }
     }
   }
@@ -482,6 +503,9 @@ static int launch_verify(const VerifyParams& prm, int B, int cl, size_t smem, cu
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
+  if (smem > 40000)
+    cudaFuncSetAttribute(verify_kernel<T, VEC, GREEDY>,
+                         cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   const cudaError_t e = cudaLaunchKernelEx(&cfg, verify_kernel<T, VEC, GREEDY>, prm);
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -607,7 +631,7 @@ extern "C" int cie_verify_drafts(const void* tokens, int64_t tokens_stride_b, in
     return aligned16(base) && (s[0] * elem) % 16 == 0 && (s[1] * elem) % 16 == 0;
   };
   const bool vec = rows16(target, target_strides) && (draft == nullptr || rows16(draft, draft_strides));
-  // as many CTAs per sequence as give every one four segments, up to a portable cluster
+  // as many CTAs per sequence as give every one a few segments, up to a portable cluster
   const int nseg = (V + kSeg - 1) / kSeg;
   int cl = 1;
   while (cl < kVfMaxCluster && nseg >= 8 * cl) cl *= 2;

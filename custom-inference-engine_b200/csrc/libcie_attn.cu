@@ -6,6 +6,7 @@
 #include "paged_attn.cu"
 #include "paged_noalloc.cu"
 #include "prefill_attn.cu"
+#include "tree_attn.cu"
 #include "int8_gemm.cu"
 #include "draft_tree.cu"
 #include "peer_barrier.cu"

@@ -76,6 +76,9 @@ struct PagedParams {
   // tree mode: parent of node i of sequence b at parents[b * par_sb + i]
   const int32_t* parents;
   int64_t par_sb;
+  // tree mode on tcgen05 (tree_attn.cu)
+  int pool_tokens;  // num_blocks * block_size: the maps' token extent
+  int o_vec;        // o's rows are 16-byte aligned
 };
 
 constexpr int kPagedWarps = 4;
@@ -1126,75 +1129,4 @@ extern "C" int cie_paged_attn(const void* q, const void* k_pool, const void* v_p
   prm.bs_log2 = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1;
   return dispatch_d<true>(prm, d, pl.mt, dtype == CIE_DTYPE_BF16,
                           reinterpret_cast<cudaStream_t>(stream));
-}
-
-// ------------------------------------------------------------------ tree of drafts
-extern "C" size_t cie_tree_attn_workspace(int B, int Hq, int Hkv, int T, int d, int block_size,
-                                          int max_blocks, int split_tokens) {
-  if (B <= 0 || Hq <= 0 || Hkv <= 0 || T <= 0 || Hq % Hkv != 0 || !mma_head_dim_ok(d) ||
-      block_size <= 0 || max_blocks < 0)
-    return 0;
-  return make_plan(B, Hq, Hkv, T, d, max_blocks * block_size, split_tokens).workspace();
-}
-
-extern "C" int cie_tree_attn(const void* q, const void* k_pool, const void* v_pool,
-                             const int32_t* block_tables, const int32_t* kv_lens,
-                             const int32_t* parents, int64_t parents_stride_b, void* o, int B,
-                             int Hq, int Hkv, int T, int d, int num_blocks, int block_size,
-                             int max_blocks, const int64_t* q_strides, const int64_t* o_strides,
-                             float scale, int dtype, const float* rope_cos, const float* rope_sin,
-                             int rope_max_pos, int split_tokens, void* workspace,
-                             size_t workspace_bytes, void* stream) {
-  CIE_CHECK_ARG(q && k_pool && v_pool && block_tables && kv_lens && parents && o,
-                "cie_tree_attn: null tensor pointer");
-  CIE_CHECK_ARG(B >= 0 && Hq > 0 && Hkv > 0 && T >= 0, "cie_tree_attn: bad shape");
-  CIE_CHECK_ARG(Hq % Hkv == 0, "cie_tree_attn: Hq (%d) must be a multiple of Hkv (%d)", Hq, Hkv);
-  CIE_CHECK_ARG(T <= CIE_MAX_TREE, "cie_tree_attn: %d nodes, at most %d", T, CIE_MAX_TREE);
-  CIE_CHECK_ARG(parents_stride_b >= 0, "cie_tree_attn: negative parents stride");
-  CIE_CHECK_ARG(dtype == CIE_DTYPE_BF16 || dtype == CIE_DTYPE_FP16, "cie_tree_attn: bad dtype %d",
-                dtype);
-  CIE_CHECK_ARG(num_blocks > 0 && block_size > 0 && max_blocks > 0,
-                "cie_tree_attn: bad pool geometry");
-  CIE_CHECK_ARG(static_cast<int64_t>(max_blocks) * block_size < (int64_t(1) << 31) - 4096,
-                "cie_tree_attn: max_blocks * block_size too large");
-  CIE_CHECK_ARG(q_strides && o_strides, "cie_tree_attn: null strides");
-  CIE_CHECK_ARG(aligned16(q) && aligned16(k_pool) && aligned16(v_pool),
-                "cie_tree_attn: q/k_pool/v_pool must be 16-byte aligned");
-  CIE_CHECK_ARG(q_strides[0] % 8 == 0 && q_strides[1] % 8 == 0 && q_strides[2] % 8 == 0,
-                "cie_tree_attn: q strides must be multiples of 8 elements");
-  CIE_CHECK_ARG(split_tokens == 0 || (split_tokens > 0 && split_tokens % 16 == 0),
-                "cie_tree_attn: split_tokens must be 0 or a positive multiple of 16");
-  CIE_CHECK_ARG((rope_cos == nullptr) == (rope_sin == nullptr),
-                "cie_tree_attn: rope_cos and rope_sin must both be given or both NULL");
-  CIE_CHECK_ARG(rope_cos == nullptr || rope_max_pos > 0, "cie_tree_attn: rope_max_pos <= 0");
-  if (!mma_head_dim_ok(d)) {
-    set_error("cie_tree_attn: head_dim %d unsupported (16, 32, 64, 128 or 256)", d);
-    return CIE_ERR_UNSUPPORTED;
-  }
-  if (B == 0 || T == 0) return CIE_OK;
-  const MmaPlan pl = make_plan(B, Hq, Hkv, T, d, max_blocks * block_size, split_tokens);
-  if (pl.workspace() > 0 && (workspace == nullptr || workspace_bytes < pl.workspace())) {
-    set_error("cie_tree_attn: workspace of %zu bytes required, got %zu", pl.workspace(),
-              workspace_bytes);
-    return CIE_ERR_WORKSPACE;
-  }
-  if (B > 65535 || static_cast<int64_t>(Hkv) * pl.row_groups > 65535) {
-    set_error("cie_tree_attn: grid too large (B=%d, Hkv*row_groups=%d)", B, Hkv * pl.row_groups);
-    return CIE_ERR_UNSUPPORTED;
-  }
-  PagedParams prm{};
-  fill_common(prm, pl, q, o, B, Hq, Hkv, T, q_strides, o_strides, scale, 0, rope_cos, rope_sin,
-              rope_max_pos, workspace);
-  prm.k_pool = k_pool;
-  prm.v_pool = v_pool;
-  prm.block_tables = block_tables;
-  prm.kv_lens = kv_lens;
-  prm.num_blocks = num_blocks;
-  prm.block_size = block_size;
-  prm.max_blocks = max_blocks;
-  prm.bs_log2 = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1;
-  prm.parents = parents;
-  prm.par_sb = parents_stride_b;
-  return dispatch_d<true, true>(prm, d, pl.mt, dtype == CIE_DTYPE_BF16,
-                                reinterpret_cast<cudaStream_t>(stream));
 }

@@ -28,16 +28,53 @@ from __future__ import annotations
 
 import ctypes
 import math
+from functools import lru_cache
 from typing import NamedTuple, Sequence
 
 import torch
 
 from kernels import _lib
-from kernels.flash_attention import _DTYPES, _kernel_ready, _require, _rope_tables
+from kernels.flash_attention import _DTYPES, _kernel_ready, _rope_tables, _require
 
 _PROB_DTYPES = {**_DTYPES, torch.float32: _lib.CIE_DTYPE_FP32}
-_I64x2 = ctypes.c_int64 * 2
-_I64x3 = ctypes.c_int64 * 3
+_I32 = torch.int32
+
+# These calls run once per layer or per token, and a small one takes the GPU less time
+# than the interpreter needs to describe it: tensors are asked for as little as the
+# checks need, and what depends on sizes alone is kept.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+@lru_cache(maxsize=4096)
+def _i64s(strides: tuple) -> ctypes.Array:
+    """The strides as a C array, read only by the library."""
+    return (ctypes.c_int64 * len(strides))(*strides)
+
+
+@lru_cache(maxsize=4096)
+def _tree_workspace(*sizes) -> int:
+    """Bytes of workspace; the last of the sizes is the device."""
+    with torch.cuda.device(sizes[-1]):
+        return _require().cie_tree_attn_workspace(*sizes[:-1])
+
+
+@lru_cache(maxsize=256)
+def _pointers(n: int):
+    """The C type of an array of n pointers (making it costs more than filling it)."""
+    return ctypes.c_void_p * n
+
+
+def _require_lib() -> ctypes.CDLL:
+    return _lib._LIB or _require()
+
+
+def _call(index: int, fn, *args) -> int:
+    """fn(*args, stream) on device ``index`` and its current stream."""
+    if index == torch.cuda.current_device():
+        return fn(*args, _raw_stream(index))
+    with torch.cuda.device(index):
+        return fn(*args, _raw_stream(index))
 
 
 class Verdict(NamedTuple):
@@ -48,19 +85,21 @@ class Verdict(NamedTuple):
     n: torch.Tensor       # (B,) int32
 
 
-def _parents(parents: torch.Tensor, B: int, T: int, device, what: str) -> tuple[torch.Tensor, int]:
+def _parents(parents: torch.Tensor, B: int, T: int, index: int, what: str
+             ) -> tuple[torch.Tensor, int]:
     """(tensor, stride between the sequences' trees)"""
-    if parents.dtype != torch.int32:
+    if parents.dtype is not _I32:
         raise ValueError(f"{what}: parents must be int32, got {parents.dtype}")
-    if parents.device != device:
+    shape = parents.shape
+    if shape != (T,) and shape != (B, T):
+        raise ValueError(f"{what}: parents must be ({T},) or ({B}, {T}), got {tuple(shape)}")
+    if parents.get_device() != index:
         raise RuntimeError(f"{what} requires all tensors on one CUDA device")
-    if parents.shape != (T,) and parents.shape != (B, T):
-        raise ValueError(f"{what}: parents must be ({T},) or ({B}, {T}), got {tuple(parents.shape)}")
     if T > _lib.CIE_MAX_TREE:
         raise ValueError(f"{what}: {T} nodes, at most {_lib.CIE_MAX_TREE}")
     if T > 1 and parents.stride(-1) != 1:
         parents = parents.contiguous()
-    return parents, (parents.stride(0) if parents.ndim == 2 and B > 1 else 0)
+    return parents, (parents.stride(0) if len(shape) == 2 and B > 1 else 0)
 
 
 def tree_attention(
@@ -86,66 +125,74 @@ def tree_attention(
     kv_lens[b] = 0. NaN or infinity in a node's K or V reaches only the nodes that
     see it.
     """
-    if not q.is_cuda:
+    index = q.get_device()
+    if index < 0:
         raise RuntimeError("tree_attention requires CUDA tensors")
     if q.ndim != 4:
         raise ValueError(f"q must be (B, Hq, T, D), got {tuple(q.shape)}")
     B, Hq, T, D = q.shape
-    if k_pool.ndim != 4 or k_pool.shape != v_pool.shape:
+    shape = k_pool.shape
+    if len(shape) != 4 or shape != v_pool.shape:
         raise ValueError("k_pool/v_pool must both be (num_blocks, block_size, Hkv, D)")
-    nb, bs, Hkv, Dk = k_pool.shape
+    nb, bs, Hkv, Dk = shape
     if Dk != D:
         raise ValueError(f"pool head_dim {Dk} != q head_dim {D}")
     if Hkv == 0 or Hq % Hkv:
         raise ValueError(f"num_heads {Hq} must be a multiple of num_kv_heads {Hkv}")
-    dtype, device = q.dtype, q.device
-    if dtype not in _DTYPES or k_pool.dtype != dtype or v_pool.dtype != dtype:
+    dtype = q.dtype
+    if dtype not in _DTYPES or k_pool.dtype is not dtype or v_pool.dtype is not dtype:
         raise ValueError(f"tree_attention expects matching FP16/BF16 q and pools, got "
                          f"{dtype}/{k_pool.dtype}/{v_pool.dtype}")
-    if block_tables.dtype != torch.int32 or kv_lens.dtype != torch.int32:
+    if block_tables.dtype is not _I32 or kv_lens.dtype is not _I32:
         raise ValueError("block_tables and kv_lens must be int32")
-    if block_tables.ndim != 2 or block_tables.shape[0] != B or kv_lens.shape != (B,):
+    tab_shape = block_tables.shape
+    if len(tab_shape) != 2 or tab_shape[0] != B or kv_lens.shape != (B,):
         raise ValueError("block_tables must be (B, max_blocks) and kv_lens (B,)")
-    if (k_pool.device != device or v_pool.device != device or block_tables.device != device
-            or kv_lens.device != device):
+    if not (k_pool.get_device() == v_pool.get_device() == block_tables.get_device()
+            == kv_lens.get_device() == index):
         raise RuntimeError("tree_attention requires all tensors on q's CUDA device")
     if not (k_pool.is_contiguous() and v_pool.is_contiguous()):
         raise ValueError("k_pool/v_pool must be contiguous")
-    if k_pool.data_ptr() % 16 or v_pool.data_ptr() % 16:
+    k_ptr, v_ptr = k_pool.data_ptr(), v_pool.data_ptr()
+    if (k_ptr | v_ptr) & 15:
         raise ValueError("k_pool/v_pool must be 16-byte aligned")
-    parents, par_sb = _parents(parents, B, T, device, "tree_attention")
+    parents, par_sb = _parents(parents, B, T, index, "tree_attention")
     if out is None:
-        out = torch.empty((B, Hq, T, D), dtype=dtype, device=device)
-    elif out.shape != (B, Hq, T, D) or out.dtype != dtype or out.device != device:
-        raise ValueError(f"out must be a ({B}, {Hq}, {T}, {D}) {dtype} tensor on {device}")
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.shape != (B, Hq, T, D) or out.dtype is not dtype or out.get_device() != index:
+        raise ValueError(f"out must be a ({B}, {Hq}, {T}, {D}) {dtype} tensor on {q.device}")
     elif out.stride(3) != 1:
         raise ValueError("out must have a unit innermost stride")
-    lib = _require()
     if B == 0 or T == 0 or Hq == 0:
         return out
-    q = _kernel_ready(q)
-    block_tables = block_tables.contiguous()
-    kv_lens = kv_lens.contiguous()
+    qs, q_ptr = q.stride(), q.data_ptr()
+    if qs[3] != 1 or (qs[0] | qs[1] | qs[2]) & 7 or q_ptr & 15:
+        q = _kernel_ready(q)
+        qs, q_ptr = q.stride(), q.data_ptr()
+    if not block_tables.is_contiguous():
+        block_tables = block_tables.contiguous()
+    if not kv_lens.is_contiguous():
+        kv_lens = kv_lens.contiguous()
     cos = sin = None
     max_pos = 0
     if rope is not None:
-        cos, sin, max_pos = _rope_tables(rope, device)
+        cos, sin, max_pos = _rope_tables(rope, q.device)
         if cos.shape[1] * 2 != D:
             raise ValueError(f"rope tables are for head_dim {cos.shape[1] * 2}, q has {D}")
-    max_blocks = block_tables.shape[1]
+        cos, sin = _kernel_ready(cos), _kernel_ready(sin)
+    max_blocks = tab_shape[1]
     split_tokens = int(split_tokens)
-    with torch.cuda.device(device):
-        ws_bytes = lib.cie_tree_attn_workspace(B, Hq, Hkv, T, D, bs, max_blocks, split_tokens)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None
-        rc = lib.cie_tree_attn(
-            q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_tables.data_ptr(),
-            kv_lens.data_ptr(), parents.data_ptr(), par_sb, out.data_ptr(), B, Hq, Hkv, T, D, nb,
-            bs, max_blocks, _I64x3(*q.stride()[:3]), _I64x3(*out.stride()[:3]),
-            1.0 / math.sqrt(D) if scale is None else float(scale), _DTYPES[dtype],
-            None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(),
-            max_pos, split_tokens, None if ws is None else ws.data_ptr(), ws_bytes,
-            torch.cuda.current_stream(device).cuda_stream)
-    _lib.check(rc, "tree_attention")
+    ws_bytes = _tree_workspace(B, Hq, Hkv, T, D, bs, max_blocks, split_tokens, index)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    rc = _call(index, _require_lib().cie_tree_attn,
+               q_ptr, k_ptr, v_ptr, block_tables.data_ptr(), kv_lens.data_ptr(),
+               parents.data_ptr(), par_sb, out.data_ptr(), B, Hq, Hkv, T, D, nb, bs, max_blocks,
+               _i64s(qs[:3]), _i64s(out.stride()[:3]),
+               1.0 / math.sqrt(D) if scale is None else float(scale), _DTYPES[dtype],
+               None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(),
+               max_pos, split_tokens, None if ws is None else ws.data_ptr(), ws_bytes)
+    if rc:
+        _lib.check(rc, "tree_attention")
     return out
 
 
@@ -179,32 +226,36 @@ def verify_drafts(
     not yet in the cache, and path[b, :n[b]] the kept nodes, root first. A row of
     probabilities without a finite positive sum gives the token -1.
     """
-    if not target_probs.is_cuda:
+    index = target_probs.get_device()
+    if index < 0:
         raise RuntimeError("verify_drafts requires CUDA tensors")
     if target_probs.ndim != 3:
         raise ValueError(f"target_probs must be (B, T, V), got {tuple(target_probs.shape)}")
     B, T, V = target_probs.shape
-    device, dtype = target_probs.device, target_probs.dtype
+    dtype = target_probs.dtype
     if T == 0 or V == 0:
         raise ValueError("verify_drafts needs at least one node and one token")
     if dtype not in _PROB_DTYPES:
         raise ValueError(f"verify_drafts expects FP32, FP16 or BF16 rows, got {dtype}")
-    if tokens.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"tokens must be int32 or int64, got {tokens.dtype}")
+    tok_type = tokens.dtype
+    if tok_type is not _I32 and tok_type is not torch.int64:
+        raise ValueError(f"tokens must be int32 or int64, got {tok_type}")
     if tokens.shape != (B, T):
         raise ValueError(f"tokens must be ({B}, {T}), got {tuple(tokens.shape)}")
-    if tokens.device != device:
+    if tokens.get_device() != index:
         raise RuntimeError("verify_drafts requires all tensors on one CUDA device")
-    parents, par_sb = _parents(parents, B, T, device, "verify_drafts")
+    parents, par_sb = _parents(parents, B, T, index, "verify_drafts")
     if T > 1 and tokens.stride(1) != 1:
         tokens = tokens.contiguous()
-    if V > 1 and target_probs.stride(2) != 1:
+    ps = target_probs.stride()
+    if ps[2] != 1 and V > 1:
         target_probs = target_probs.contiguous()
+        ps = target_probs.stride()
     u_ptr, u_sb, q_ptr, q_strides, Td = None, 0, None, None, 0
     if uniforms is not None:
-        if uniforms.dtype != torch.float32 or uniforms.shape != (B, T):
+        if uniforms.dtype is not torch.float32 or uniforms.shape != (B, T):
             raise ValueError(f"uniforms must be a ({B}, {T}) float32 tensor")
-        if uniforms.device != device:
+        if uniforms.get_device() != index:
             raise RuntimeError("verify_drafts requires all tensors on one CUDA device")
         if T > 1 and uniforms.stride(1) != 1:
             uniforms = uniforms.contiguous()
@@ -212,31 +263,28 @@ def verify_drafts(
     if draft_probs is not None:
         if uniforms is None:
             raise ValueError("draft_probs are for sampling: pass uniforms too")
-        if draft_probs.ndim != 3 or draft_probs.shape[0] != B or draft_probs.shape[2] != V \
-                or not 1 <= draft_probs.shape[1] <= T:
-            raise ValueError(f"draft_probs must be ({B}, 1..{T}, {V}), got "
-                             f"{tuple(draft_probs.shape)}")
-        if draft_probs.dtype != dtype:
+        qshape = draft_probs.shape
+        if len(qshape) != 3 or qshape[0] != B or qshape[2] != V or not 1 <= qshape[1] <= T:
+            raise ValueError(f"draft_probs must be ({B}, 1..{T}, {V}), got {tuple(qshape)}")
+        if draft_probs.dtype is not dtype:
             raise ValueError(f"draft_probs must be {dtype} like target_probs")
-        if draft_probs.device != device:
+        if draft_probs.get_device() != index:
             raise RuntimeError("verify_drafts requires all tensors on one CUDA device")
-        if V > 1 and draft_probs.stride(2) != 1:
+        if draft_probs.stride(2) != 1 and V > 1:
             draft_probs = draft_probs.contiguous()
-        Td = draft_probs.shape[1]
-        q_ptr, q_strides = draft_probs.data_ptr(), _I64x2(*draft_probs.stride()[:2])
-    lib = _require()
-    out = torch.empty((B, T), dtype=tokens.dtype, device=device)
-    path = torch.empty((B, T), dtype=torch.int32, device=device)
-    n = torch.empty((B,), dtype=torch.int32, device=device)
-    if B == 0:
-        return Verdict(out, path, n)
-    with torch.cuda.device(device):
-        rc = lib.cie_verify_drafts(
-            tokens.data_ptr(), tokens.stride(0), tokens.dtype == torch.int64, parents.data_ptr(),
-            par_sb, target_probs.data_ptr(), _I64x2(*target_probs.stride()[:2]), q_ptr, q_strides,
-            Td, u_ptr, u_sb, B, T, V, _PROB_DTYPES[dtype], out.data_ptr(), path.data_ptr(),
-            n.data_ptr(), torch.cuda.current_stream(device).cuda_stream)
-    _lib.check(rc, "verify_drafts")
+        Td = qshape[1]
+        q_ptr, q_strides = draft_probs.data_ptr(), _i64s(draft_probs.stride()[:2])
+    out = torch.empty_like(tokens, memory_format=torch.contiguous_format)
+    path = torch.empty_like(out, dtype=_I32)
+    n = path.new_empty(B)
+    if B:
+        rc = _call(index, _require_lib().cie_verify_drafts,
+                   tokens.data_ptr(), tokens.stride(0), tok_type is torch.int64,
+                   parents.data_ptr(), par_sb, target_probs.data_ptr(), _i64s(ps[:2]), q_ptr,
+                   q_strides, Td, u_ptr, u_sb, B, T, V, _PROB_DTYPES[dtype], out.data_ptr(),
+                   path.data_ptr(), n.data_ptr())
+        if rc:
+            _lib.check(rc, "verify_drafts")
     return Verdict(out, path, n)
 
 
@@ -256,18 +304,18 @@ def keep_path(
     base = kv_lens[b] - T. Rows elsewhere stay as they are. Returns the new
     lengths, max(0, base + n[b]), int32 (B,).
     """
-    if path.ndim != 2 or path.dtype != torch.int32:
-        raise ValueError("path must be int32 (B, T)")
-    if not path.is_cuda:
+    index = path.get_device()
+    if index < 0:
         raise RuntimeError("keep_path requires CUDA tensors")
+    if path.ndim != 2 or path.dtype is not _I32:
+        raise ValueError("path must be int32 (B, T)")
     B, T = path.shape
-    device = path.device
-    if block_tables.dtype != torch.int32 or kv_lens.dtype != torch.int32 or n.dtype != torch.int32:
+    if block_tables.dtype is not _I32 or kv_lens.dtype is not _I32 or n.dtype is not _I32:
         raise ValueError("block_tables, kv_lens and n must be int32")
     if block_tables.ndim != 2 or block_tables.shape[0] != B or kv_lens.shape != (B,) \
             or n.shape != (B,):
         raise ValueError("block_tables must be (B, max_blocks), kv_lens and n (B,)")
-    if block_tables.device != device or kv_lens.device != device or n.device != device:
+    if not block_tables.get_device() == kv_lens.get_device() == n.get_device() == index:
         raise RuntimeError("keep_path requires all tensors on one CUDA device")
     if not 1 <= T <= _lib.CIE_MAX_TREE:
         raise ValueError(f"keep_path: {T} nodes, 1 to {_lib.CIE_MAX_TREE} are served")
@@ -279,21 +327,21 @@ def keep_path(
     if dtype not in _DTYPES:
         raise ValueError(f"keep_path expects FP16/BF16 pools, got {dtype}")
     for p in pools:
-        if p.shape != shape or p.dtype != dtype or not p.is_contiguous():
+        if p.dtype is not dtype or p.shape != shape or not p.is_contiguous():
             raise ValueError("pools must be contiguous and of one shape and dtype")
-        if p.device != device:
+        if p.get_device() != index:
             raise RuntimeError("keep_path requires all tensors on one CUDA device")
-    lib = _require()
-    new_lens = torch.empty((B,), dtype=torch.int32, device=device)
+    new_lens = torch.empty_like(kv_lens, memory_format=torch.contiguous_format)
     if B == 0:
         return new_lens
-    block_tables = block_tables.contiguous()
+    if not block_tables.is_contiguous():
+        block_tables = block_tables.contiguous()
     kv_lens, path, n = kv_lens.contiguous(), path.contiguous(), n.contiguous()
-    ptrs = (ctypes.c_void_p * len(pools))(*[p.data_ptr() for p in pools])
-    with torch.cuda.device(device):
-        rc = lib.cie_keep_path(
-            ptrs, len(pools), block_tables.data_ptr(), kv_lens.data_ptr(), path.data_ptr(),
-            n.data_ptr(), new_lens.data_ptr(), B, T, shape[0], shape[1], block_tables.shape[1],
-            shape[2] * shape[3] * 2, torch.cuda.current_stream(device).cuda_stream)
-    _lib.check(rc, "keep_path")
+    ptrs = _pointers(len(pools))(*[p.data_ptr() for p in pools])
+    rc = _call(index, _require_lib().cie_keep_path,
+               ptrs, len(pools), block_tables.data_ptr(), kv_lens.data_ptr(), path.data_ptr(),
+               n.data_ptr(), new_lens.data_ptr(), B, T, shape[0], shape[1],
+               block_tables.shape[1], shape[2] * shape[3] * 2)
+    if rc:
+        _lib.check(rc, "keep_path")
     return new_lens

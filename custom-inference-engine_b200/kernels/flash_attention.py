@@ -335,7 +335,9 @@ def rope_append(
     if parents is not None:
         from kernels.draft_tree import _parents
 
-        parents, par_sb = _parents(parents, B, L, k_new.device, "rope_append")
+        parents, par_sb = _parents(parents, B, L, k_new.get_device(), "rope_append")
+        if cos is not None and cos.shape[1] * 2 != D:
+            raise ValueError(f"rope tables are for head_dim {cos.shape[1] * 2}, k has {D}")
         with torch.cuda.device(k_new.device):
             rc = lib.cie_rope_append_tree(
                 _vp(k_new), _vp(v_new), _vp(k_pool), _vp(v_pool), _vp(block_tables.contiguous()),

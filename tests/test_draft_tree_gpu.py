@@ -130,6 +130,20 @@ def test_tree_attention_shared_tree():
     check(s)
 
 
+@pytest.mark.parametrize("D,T,Hq", [(128, 32, 32), (64, 12, 32), (64, 48, 32), (128, 40, 64)])
+def test_tree_attention_many_units(D, T, Hq):
+    """More work than fits on the GPU at once, in ragged sequences: every pipeline wait ends (the
+    status word stays clear) and repeated calls agree bit for bit."""
+    rs = np.random.RandomState(D + T)
+    s = setup(32, T, Hq, 8, D, 16, BF16, [int(x) for x in rs.randint(T, 6000, 32)], seed=21)
+    out = run(s)
+    for _ in range(10):
+        assert torch.equal(run(s), out)
+    pick = [0, 13, 31]
+    ref, bound = tree_attention_ref(s["q"][pick], s["k"], s["v"], s["tables"][pick], s["lens"][pick], s["parents"][pick])
+    assert_within(out[pick], ref, bound)
+
+
 @pytest.mark.parametrize("D,Hq,Hkv,T", [(64, 8, 2, 6), (128, 8, 2, 40), (32, 4, 4, 6)])
 def test_tree_attention_idle_and_short_sequences(D, Hq, Hkv, T):
     """A sequence of length 0 gives zeros; one shorter than the tree has no slots for its first nodes."""
