@@ -30,7 +30,7 @@ from dataclasses import dataclass
 import torch
 
 from engine.cache.block_table import BlockTable
-from engine.cache.kv_cache import PagedKVCache
+from engine.cache.kv_cache import PagedKVCache, _to_device
 
 # Query rows per kv head up to which the paged split-KV kernel serves a call;
 # longer query blocks (prefill) go to the tcgen05 prefill kernel.
@@ -135,14 +135,48 @@ class BatchStep:
     block_tables: torch.Tensor    # int32 (B, max_blocks) on the cache's device
     kv_lens: torch.Tensor         # int32 (B,) lengths after the step
     start_pos: torch.Tensor       # int32 (B,) = starts, on the device
+    # int32 (new_tokens,) or (B, new_tokens): the new tokens are the nodes of a tree of
+    # drafts (kernels.draft_tree) instead of a chain
+    parents: torch.Tensor | None = None
 
 
-def begin_step(cache: PagedKVCache, tables: list[BlockTable], new_tokens: int) -> BatchStep:
-    """Reserve ``new_tokens`` positions at the end of every table and pack the tables."""
+def _tree_parents(parents, batch: int, nodes: int) -> torch.Tensor:
+    """int32 (nodes,) or (batch, nodes) from lists, checked: node 0 the root, every
+    other node's parent below it, -1 for padding."""
+    t = torch.as_tensor(parents, dtype=torch.int32)
+    if t.shape != (nodes,) and t.shape != (batch, nodes):
+        raise ValueError(f"parents must be ({nodes},) or ({batch}, {nodes}), got "
+                         f"{tuple(t.shape)}")
+    at = torch.arange(nodes, dtype=torch.int32)
+    if bool((t >= at).any()) or bool((t < -1).any()):
+        raise ValueError("a node's parent must be an earlier node, or -1")
+    return t
+
+
+def begin_step(cache: PagedKVCache, tables: list[BlockTable], new_tokens: int,
+               parents=None) -> BatchStep:
+    """Reserve ``new_tokens`` positions at the end of every table and pack the tables.
+
+    parents: the new tokens of every sequence are a tree of drafts instead of a chain:
+    its root, the last decided token, and the drafted nodes, each with the index of its
+    parent (-1 for the root and for padding). One list for the batch or one per
+    sequence, checked here, or an int32 CUDA tensor of either shape, used as it is
+    (trees made on the device; the kernels report bad entries in the status word).
+    After the layers, :func:`end_tree_step` keeps the verified path.
+    """
     if not tables:
         raise ValueError("begin_step needs at least one sequence")
     if new_tokens <= 0:
         raise ValueError(f"new_tokens must be positive, got {new_tokens}")
+    if parents is not None:
+        if not (isinstance(parents, torch.Tensor) and parents.is_cuda):
+            parents = _tree_parents(parents, len(tables), new_tokens)
+            parents = _to_device(parents, cache.device)
+        elif parents.dtype != torch.int32 or parents.shape not in (
+                (new_tokens,), (len(tables), new_tokens)):
+            raise ValueError(f"parents must be int32 ({new_tokens},) or "
+                             f"({len(tables)}, {new_tokens}), got {parents.dtype} "
+                             f"{tuple(parents.shape)}")
     starts = [t.length for t in tables]
     for t, s in zip(tables, starts):
         cache.alloc.reserve(t, s + new_tokens)
@@ -152,7 +186,27 @@ def begin_step(cache: PagedKVCache, tables: list[BlockTable], new_tokens: int) -
     if torch.device(cache.device).type == "cuda":
         start_pos = start_pos.pin_memory().to(cache.device, non_blocking=True)
     return BatchStep(tables=list(tables), new_tokens=new_tokens, starts=starts,
-                     block_tables=tab, kv_lens=lens, start_pos=start_pos)
+                     block_tables=tab, kv_lens=lens, start_pos=start_pos, parents=parents)
+
+
+def end_tree_step(cache: PagedKVCache, step: BatchStep, verdict) -> list[list[int]]:
+    """Keep what :func:`kernels.draft_tree.verify_drafts` decided about a tree step.
+
+    The kept nodes' K/V move behind each history, in all layers, and the tables shrink
+    to them. Returns each sequence's new tokens; the last is not in the cache yet and is
+    the root of the next tree. Reading them is the step's only host sync.
+    """
+    if step.parents is None:
+        raise ValueError("end_tree_step ends a step that begin_step began with parents")
+    B, T = len(step.tables), step.new_tokens
+    if verdict.path.shape != (B, T) or verdict.tokens.shape != (B, T):
+        raise ValueError(f"the verdict is for {tuple(verdict.path.shape)} (sequences, nodes), "
+                         f"the step for ({B}, {T})")
+    cache.keep_path(step.block_tables, step.kv_lens, verdict.path, verdict.n)
+    both = torch.cat([verdict.n[:, None].to(verdict.tokens.dtype), verdict.tokens], 1).tolist()
+    for table, start, row in zip(step.tables, step.starts, both):
+        cache.rollback(table, start + row[0])
+    return [row[1:1 + row[0]] for row in both]
 
 
 def attention_forward_batch(
@@ -174,6 +228,9 @@ def attention_forward_batch(
     history is empty, else reading each sequence's history through the block
     table (block sizes that are multiples of 16, d 64 / 128; other geometries
     gather each history and launch per sequence). Returns (B, Hq, L, d).
+
+    A step with ``parents`` has a tree of drafts as its new tokens: K and q are rotated
+    at start + depth, and every node attends over the history and its ancestors.
     """
     from kernels.flash_attention import flash_attention as _fa
     from kernels.flash_attention import paged_attention, rope_append
@@ -188,7 +245,12 @@ def attention_forward_batch(
     if scale is None:
         scale = 1.0 / math.sqrt(d)
     rope_append(k.transpose(1, 2), v.transpose(1, 2), cache.k[layer_idx], cache.v[layer_idx],
-                step.block_tables, step.start_pos, rope=rope)
+                step.block_tables, step.start_pos, rope=rope, parents=step.parents)
+    if step.parents is not None:
+        from kernels.draft_tree import tree_attention
+
+        return tree_attention(q, cache.k[layer_idx], cache.v[layer_idx], step.block_tables,
+                              step.kv_lens, step.parents, scale, rope=rope)
     if (Hq // Hkv) * L <= PAGED_MAX_ROWS:
         return paged_attention(q, cache.k[layer_idx], cache.v[layer_idx], step.block_tables,
                                step.kv_lens, True, scale, rope=rope)

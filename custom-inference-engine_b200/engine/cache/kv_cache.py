@@ -11,6 +11,8 @@ free with the same semantics. The data path is native:
 * ``gather`` is the bit-exact ``gather_kv`` kernel;
 * ``device_tables`` packs several sequences' block lists into the int32
   (B, max_blocks) table + (B,) lengths that ``paged_attention`` reads;
+* ``keep_path`` moves the verified path of a tree of drafts behind the history, in
+  every layer's pools with one launch;
 * ``fork`` copies the blocks with the ``copy_blocks`` kernel (one launch per
   pool) instead of an index_select + index_copy_ per layer.
 
@@ -182,6 +184,16 @@ class PagedKVCache:
                                      block_bytes, _stream(self.k[0]))
             _lib.check(rc, "fork")
         return BlockTable(block_size=self.cfg.block_size, blocks=new_blocks, length=table.length)
+
+    def keep_path(self, block_tables: torch.Tensor, kv_lens: torch.Tensor, path: torch.Tensor,
+                  n: torch.Tensor) -> torch.Tensor:
+        """Move the kept nodes of each sequence's tree of drafts, its last slots, behind
+        the history, in every layer's pools at once (``kernels.draft_tree.keep_path``);
+        returns the new lengths, int32 (B,), on the device. The host tables shrink with
+        ``rollback`` once those are known."""
+        from kernels.draft_tree import keep_path
+
+        return keep_path(self.k + self.v, block_tables, kv_lens, path, n)
 
     def rollback(self, table: BlockTable, new_length: int) -> None:
         self.alloc.rollback(table, new_length)

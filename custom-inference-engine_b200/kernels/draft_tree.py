@@ -29,6 +29,7 @@ from __future__ import annotations
 import ctypes
 import math
 from functools import lru_cache
+from operator import attrgetter
 from typing import NamedTuple, Sequence
 
 import torch
@@ -38,6 +39,7 @@ from kernels.flash_attention import _DTYPES, _kernel_ready, _rope_tables, _requi
 
 _PROB_DTYPES = {**_DTYPES, torch.float32: _lib.CIE_DTYPE_FP32}
 _I32 = torch.int32
+_SHAPE_AND_TYPE = attrgetter("shape", "dtype")
 
 # These calls run once per layer or per token, and a small one takes the GPU less time
 # than the interpreter needs to describe it: tensors are asked for as little as the
@@ -326,18 +328,18 @@ def keep_path(
         raise ValueError("pools must be (num_blocks, block_size, Hkv, D)")
     if dtype not in _DTYPES:
         raise ValueError(f"keep_path expects FP16/BF16 pools, got {dtype}")
-    for p in pools:
-        if p.dtype is not dtype or p.shape != shape or not p.is_contiguous():
-            raise ValueError("pools must be contiguous and of one shape and dtype")
-        if p.get_device() != index:
-            raise RuntimeError("keep_path requires all tensors on one CUDA device")
+    if set(map(_SHAPE_AND_TYPE, pools)) != {(shape, dtype)} \
+            or not all(map(torch.Tensor.is_contiguous, pools)):
+        raise ValueError("pools must be contiguous and of one shape and dtype")
+    if set(map(torch.Tensor.get_device, pools)) != {index}:
+        raise RuntimeError("keep_path requires all tensors on one CUDA device")
     new_lens = torch.empty_like(kv_lens, memory_format=torch.contiguous_format)
     if B == 0:
         return new_lens
     if not block_tables.is_contiguous():
         block_tables = block_tables.contiguous()
     kv_lens, path, n = kv_lens.contiguous(), path.contiguous(), n.contiguous()
-    ptrs = _pointers(len(pools))(*[p.data_ptr() for p in pools])
+    ptrs = _pointers(len(pools))(*map(torch.Tensor.data_ptr, pools))
     rc = _call(index, _require_lib().cie_keep_path,
                ptrs, len(pools), block_tables.data_ptr(), kv_lens.data_ptr(), path.data_ptr(),
                n.data_ptr(), new_lens.data_ptr(), B, T, shape[0], shape[1],

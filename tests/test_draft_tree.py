@@ -139,3 +139,17 @@ def test_reference_restatement():
     # chosen drafts: 0.6 < 0.3 no; then 0.2 < m = 0.7 times u = 0.2: kept
     assert verify_ref(tok, tree, p, torch.tensor([[0.0, 0.6, 0.2]])) == ([[2, 0, -1]], [[0, 2, -1]], [2])
     assert verify_ref(torch.tensor([[9, 0, 0]]), torch.tensor([-1, 0, 1]), p) == ([[0, 0, 0]], [[0, 1, 2]], [3])
+
+
+def test_step_checks_trees():
+    from engine.attention import _tree_parents, end_tree_step, BatchStep
+
+    assert _tree_parents([-1, 0, 1], 2, 3).tolist() == [-1, 0, 1]
+    assert _tree_parents([[-1, 0, 1], [-1, 0, -1]], 2, 3).dtype == torch.int32
+    for bad, text in (([-1, 0], "parents must be"), ([-1, 1, 0], "earlier"), ([-1, 0, -2], "earlier"), ([0, 0, 0], "earlier"),
+                      ([[-1, 0, 1]] * 3, "parents must be")):
+        with pytest.raises(ValueError, match=text):
+            _tree_parents(bad, 2, 3)
+    step = BatchStep([], 1, [], None, None, None)
+    with pytest.raises(ValueError, match="parents"):
+        end_tree_step(None, step, None)

@@ -535,3 +535,114 @@ def test_keep_path_idle_and_bad_entries(cuda):
     keep_path(pools, tables, s["lens"], good.cuda(), torch.tensor([1, 2, 1], dtype=torch.int32, device="cuda"))
     assert _lib.device_status() == _lib.CIE_DEV_BAD_BLOCK_ID
     assert torch.equal(now, pools[0])
+
+
+# ------------------------------------------------------------------ together
+def _model(layers, hq, hkv, d, vocab, seed):
+    """A small attention-only model in 64 bits and its weights in bf16."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    dim = hq * d
+    r = lambda *s: (torch.randn(*s, generator=gen, device="cuda") * s[0] ** -0.5).to(BF16)  # noqa: E731
+    return dict(embed=(torch.randn(vocab, dim, generator=gen, device="cuda")).to(BF16), head=r(dim, vocab),
+                layers=[dict(q=r(dim, hq * d), k=r(dim, hkv * d), v=r(dim, hkv * d), o=r(dim, dim)) for _ in range(layers)])
+
+
+def _forward(m, cache, step, tokens, hq, hkv, d, rope):
+    from engine.attention import attention_forward_batch
+
+    B, T = tokens.shape
+    x = m["embed"][tokens]
+    for i, w in enumerate(m["layers"]):
+        heads = lambda n, h: (x @ w[n]).view(B, T, h, d).transpose(1, 2)  # noqa: E731,B023
+        a = attention_forward_batch(heads("q", hq), heads("k", hkv), heads("v", hkv), cache, i, step, rope=rope)
+        x = x + a.transpose(1, 2).reshape(B, T, hq * d) @ w["o"]
+    return x.float() @ m["head"].float()
+
+
+@pytest.mark.parametrize("hq,hkv,d,bs", [(8, 2, 64, 16), (4, 4, 32, 8)])
+def test_tree_steps_decode_like_chains(hq, hkv, d, bs):
+    """Greedy decoding by trees of drafts, one of whose paths is right: the cache after every
+    step holds the rows that plain decoding of the same tokens appends, and the tokens are its tokens."""
+    from engine.attention import attention_forward_batch, begin_step, end_tree_step
+    from engine.cache import KVCacheConfig, PagedKVCache
+    from kernels.draft_tree import verify_drafts
+
+    layers, vocab, B = 3, 97, 3
+    m = _model(layers, hq, hkv, d, vocab, 1)
+    rope = rope_tables(d)
+    mk = lambda: PagedKVCache(KVCacheConfig(num_layers=layers, num_kv_heads=hkv, head_dim=d, num_blocks=80, block_size=bs))  # noqa: E731
+    plain, treed = mk(), mk()
+    pt, tt = [plain.new_sequence() for _ in range(B)], [treed.new_sequence() for _ in range(B)]
+    rs = np.random.RandomState(3)
+    prompt = torch.from_numpy(rs.randint(0, vocab, (B, 9))).cuda()
+    first = []
+    for cache, tables in ((plain, pt), (treed, tt)):
+        first.append(_forward(m, cache, begin_step(cache, tables, 9), prompt, hq, hkv, d, rope)[:, -1].argmax(-1))
+    assert torch.equal(*first)
+    # plain greedy decoding
+    want, last = [[] for _ in range(B)], first[0]
+    for _ in range(14):
+        for b in range(B):
+            want[b].append(int(last[b]))
+        last = _forward(m, plain, begin_step(plain, pt, 1), last[:, None], hq, hkv, d, rope)[:, -1].argmax(-1)
+    for b in range(B):
+        want[b].append(int(last[b]))
+    got, sizes = [[int(first[0][b])] for b in range(B)], []
+    parents = [[-1, 0, 0, 1, 2, 2, 4, 6], [-1, 0, 1, 2, 3, 4, 5, 6], [-1, 0, 0, 0, 3, 4, 4, -1]]
+    good = [[2, 5], [1, 2, 3, 4], [3, 4, 6]]  # nodes that draft what plain decoding finds next
+    while min(len(g) for g in got) < 8:
+        tokens = torch.from_numpy(rs.randint(0, vocab, (B, 8))).cuda()
+        for b in range(B):
+            tokens[b, 0] = got[b][-1]
+            for k, node in enumerate(good[b]):
+                tokens[b, node] = want[b][len(got[b]) + k]
+        step = begin_step(treed, tt, 8, parents=parents)
+        logits = _forward(m, treed, step, tokens, hq, hkv, d, rope)
+        verdict = verify_drafts(tokens, step.parents, logits)
+        new = end_tree_step(treed, step, verdict)
+        for b in range(B):
+            assert len(new[b]) >= len(good[b]) + 1 or new[b] == want[b][len(got[b]):len(got[b]) + len(new[b])]
+            got[b] += new[b]
+        sizes.append([len(n) for n in new])
+        assert [t.length for t in tt] == [9 + len(g) - 1 for g in got]
+    for b in range(B):
+        n = min(len(got[b]), len(want[b]))
+        assert got[b][:n] == want[b][:n], (sizes, got[b], want[b])
+        rows = 9 + min(len(got[b]), len(want[b])) - 1
+        for layer in range(layers):
+            for x, y in zip(plain.gather(layer, pt[b]), treed.gather(layer, tt[b])):
+                # the first layer's rows do not depend on attention: the same bits
+                if layer == 0:
+                    assert torch.equal(x[:rows], y[:rows])
+                else:
+                    assert float((x[:rows].float() - y[:rows].float()).abs().max()) < 0.1
+
+
+def test_tree_step_has_no_host_sync_before_its_end():
+    from engine.attention import attention_forward_batch, begin_step
+    from engine.cache import KVCacheConfig, PagedKVCache
+    from kernels.draft_tree import verify_drafts
+
+    cache = PagedKVCache(KVCacheConfig(num_layers=2, num_kv_heads=2, head_dim=64, num_blocks=64, block_size=16))
+    tables = [cache.new_sequence() for _ in range(2)]
+    rope = rope_tables(64)
+    rnd = lambda h, n: torch.randn(2, h, n, 64, device="cuda", dtype=BF16)  # noqa: E731
+    p, q, u = probs(2, 6, 512, 1)
+    parents = torch.tensor([-1, 0, 0, 1, 1, 2], dtype=torch.int32, device="cuda")
+    tokens = drafted(q, parents, 2)
+
+    def step_once():
+        s = begin_step(cache, tables, 6, parents=parents)
+        for layer in range(2):
+            attention_forward_batch(rnd(8, 6), rnd(2, 6), rnd(2, 6), cache, layer, s, rope=rope)
+        v = verify_drafts(tokens, parents, p, u, q)
+        return s, cache.keep_path(s.block_tables, s.kv_lens, v.path, v.n), v
+
+    step_once()
+    torch.cuda.synchronize()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        s, lens, v = step_once()
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    assert lens.tolist() == [6 + n for n in v.n.tolist()]
