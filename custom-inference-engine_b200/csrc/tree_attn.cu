@@ -90,14 +90,14 @@ struct TcPlan {
 
 __device__ __forceinline__ int tc_places(int tiles) { return tiles > 0 ? tiles + kTcOpen : 0; }
 
-// mine: the places of sequence `lane`.
+// len: the length of sequence `lane` (0 past the last), loaded early; mine: its places.
 __device__ __forceinline__ TcPlan tc_plan(const PagedParams& p, int keys, int parts, int lane,
-                                          int& mine) {
-  int sum = 0, most = 0;
-  mine = 0;
-  for (int b = lane; b < p.B; b += 32) {
+                                          int len, int& mine) {
+  int most = (len + keys - 1) / keys;
+  mine = tc_places(most);
+  int sum = mine;
+  for (int b = lane + 32; b < p.B; b += 32) {
     const int tiles = (tc_len(p, b) + keys - 1) / keys;
-    if (b == lane) mine = tc_places(tiles);
     sum += tc_places(tiles);
     most = max(most, tiles);
   }
@@ -144,10 +144,11 @@ struct TcWalk {
     }
     more = false;
   }
-  __device__ __forceinline__ void start(const PagedParams& p, int keys, int groups, int lane) {
+  __device__ __forceinline__ void start(const PagedParams& p, int keys, int groups, int lane,
+                                        int len) {
     const int parts = gridDim.x / groups, part = blockIdx.x / groups;
     int mine;
-    const TcPlan plan = tc_plan(p, keys, parts, lane, mine);
+    const TcPlan plan = tc_plan(p, keys, parts, lane, len, mine);
     whole = plan.whole;
     more = true;
     first = 0;
@@ -218,6 +219,8 @@ __global__ void __launch_bounds__(kTcThreads, 2)
   const int groups = p.Hkv * p.row_groups;
   const int R = p.G * p.M;
 
+  const int len = lane < p.B ? tc_len(p, lane) : 0;  // on its way during the set-up
+
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -270,7 +273,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
 
   if (warp < 4) {
     TcWalk w;
-    if (warp != 3) w.start(p, KEYS, groups, lane);
+    if (warp != 3) w.start(p, KEYS, groups, lane, len);
     if (warp == 0 || warp == 2) {
       // ---------------------------------------------- loaders
       const bool is_k = warp == 0;
@@ -422,20 +425,19 @@ __global__ void __launch_bounds__(kTcThreads, 2)
       const uint32_t lanes = static_cast<uint32_t>(wq * 32) << 16;
       const uint32_t o_col = tmem + lanes + C::TM_O;
       const int words = tree_words(p.M);
-      TcWalk w, ahead;
-      w.start(p, KEYS, groups, lane);
-
       const int gr = row0 + row;
       const bool live_row = gr < R;
       const int node = live_row ? gr % p.M : 0;
       const int head = kvh * p.G + (live_row ? gr / p.M : 0);
+      const int64_t q_off = head * p.q_sh + node * p.q_sm;  // of this lane's row
+      const uint32_t live_rows = __ballot_sync(0xffffffffu, live_row);
+      TcWalk w, ahead;
+      w.start(p, KEYS, groups, lane, len);
 
       // Q rows and parents of piece number k, `x`, on their way to shared memory: a warp
       // copies its 32 rows, whole rows at a time (a row per lane would touch 32 lines
       // with every instruction), and all parents, as the other warps do, the same values
       // to the same place.
-      const int64_t q_off = head * p.q_sh + node * p.q_sm;  // of this lane's row
-      const uint32_t live_rows = __ballot_sync(0xffffffffu, live_row);
       auto fetch = [&](const TcWalk& x, int k) {
         constexpr int CPR = D / 8, RPI = 32 / CPR;  // 16-byte chunks of a row, rows at a time
         const int ch = lane % CPR;
@@ -797,7 +799,8 @@ __global__ void __launch_bounds__(kTcMergeThreads)
   const int groups = p.Hkv * p.row_groups;
   const int b = blockIdx.x / groups, y = blockIdx.x % groups;
   int mine;
-  const TcPlan plan = tc_plan(p, keys, ctas / groups, lane, mine);
+  const TcPlan plan =
+      tc_plan(p, keys, ctas / groups, lane, lane < p.B ? tc_len(p, lane) : 0, mine);
   const int tiles = (tc_len(p, b) + keys - 1) / keys;
   int at = 0;  // the sequence's place in the list
   if (lane < b) at = mine;
@@ -814,20 +817,39 @@ __global__ void __launch_bounds__(kTcMergeThreads)
   auto row_of = [&](int part) {
     return static_cast<int64_t>(2 * (part * groups + y) + (part == c0 ? 1 : 0)) * p.rg_rows + r;
   };
-  float mx = -INFINITY;
-#pragma unroll 8
-  for (int i = c0; i <= c1; ++i) mx = fmaxf(mx, __ldg(p.part_lse + row_of(i)));
-  float sum = 0.f;
+  // eight pieces at a time, their loads in flight together; a NaN weight stays NaN
+  float mx = -INFINITY, sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-  for (int i = c0; i <= c1; ++i) {
-    const float wt = mx == -INFINITY ? 0.f : ex2(__ldg(p.part_lse + row_of(i)) - mx);
-    const float4 v = __ldg(reinterpret_cast<const float4*>(p.part_o + row_of(i) * D) + c);
-    sum += wt;
-    acc.x += wt * v.x;
-    acc.y += wt * v.y;
-    acc.z += wt * v.z;
-    acc.w += wt * v.w;
+  for (int i0 = c0; i0 <= c1; i0 += 8) {
+    float lse[8];
+    float4 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const bool there = i0 + i <= c1;
+      lse[i] = there ? __ldg(p.part_lse + row_of(i0 + i)) : -INFINITY;
+      v[i] = there ? __ldg(reinterpret_cast<const float4*>(p.part_o + row_of(i0 + i) * D) + c)
+                   : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float top = mx;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, lse[i]);
+    if (top == -INFINITY) top = 0.f;  // nothing so far: all weights 0 (or NaN)
+    const float old = ex2(mx - top);
+    sum *= old;
+    acc.x *= old;
+    acc.y *= old;
+    acc.z *= old;
+    acc.w *= old;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float wt = ex2(lse[i] - top);
+      sum += wt;
+      acc.x += wt * v[i].x;
+      acc.y += wt * v[i].y;
+      acc.z += wt * v[i].z;
+      acc.w += wt * v[i].w;
+    }
+    mx = top;
   }
   const float inv = sum > 0.f ? 1.0f / sum : __int_as_float(0x7fc00000);
   using elem_t = typename std::conditional<BF16, __nv_bfloat16, __half>::type;

@@ -66,7 +66,7 @@ SIGNATURES: dict[str, tuple] = {
     "cie_tree_attn_workspace": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i]),
     "cie_verify_drafts": (_i, [_vp, _i64, _i, _vp, _i64, _vp, _i64p, _vp, _i64p, _i, _vp, _i64, _i,
                                _i, _i, _i, _vp, _vp, _vp, _vp]),
-    "cie_keep_path": (_i, [ctypes.POINTER(_vp), _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i,
+    "cie_keep_path": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i,
                            _sz, _vp]),
     "cie_copy_blocks": (_i, [ctypes.POINTER(_vp), _i, _vp, _vp, _i, _i, _sz, _vp]),
     "cie_rope": (_i, [_vp, _vp, _i, _i, _i, _i, _i64p, _i64p, _i, _i, _vp, _vp, _i, _vp]),

@@ -28,6 +28,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from array import array
 from functools import lru_cache
 from operator import attrgetter
 from typing import NamedTuple, Sequence
@@ -39,7 +40,7 @@ from kernels.flash_attention import _DTYPES, _kernel_ready, _rope_tables, _requi
 
 _PROB_DTYPES = {**_DTYPES, torch.float32: _lib.CIE_DTYPE_FP32}
 _I32 = torch.int32
-_SHAPE_AND_TYPE = attrgetter("shape", "dtype")
+_SHAPE, _DTYPE = attrgetter("shape"), attrgetter("dtype")
 
 # These calls run once per layer or per token, and a small one takes the GPU less time
 # than the interpreter needs to describe it: tensors are asked for as little as the
@@ -59,12 +60,6 @@ def _tree_workspace(*sizes) -> int:
     """Bytes of workspace; the last of the sizes is the device."""
     with torch.cuda.device(sizes[-1]):
         return _require().cie_tree_attn_workspace(*sizes[:-1])
-
-
-@lru_cache(maxsize=256)
-def _pointers(n: int):
-    """The C type of an array of n pointers (making it costs more than filling it)."""
-    return ctypes.c_void_p * n
 
 
 def _require_lib() -> ctypes.CDLL:
@@ -328,7 +323,8 @@ def keep_path(
         raise ValueError("pools must be (num_blocks, block_size, Hkv, D)")
     if dtype not in _DTYPES:
         raise ValueError(f"keep_path expects FP16/BF16 pools, got {dtype}")
-    if set(map(_SHAPE_AND_TYPE, pools)) != {(shape, dtype)} \
+    if list(map(_SHAPE, pools)).count(shape) != len(pools) \
+            or set(map(_DTYPE, pools)) != {dtype} \
             or not all(map(torch.Tensor.is_contiguous, pools)):
         raise ValueError("pools must be contiguous and of one shape and dtype")
     if set(map(torch.Tensor.get_device, pools)) != {index}:
@@ -339,9 +335,9 @@ def keep_path(
     if not block_tables.is_contiguous():
         block_tables = block_tables.contiguous()
     kv_lens, path, n = kv_lens.contiguous(), path.contiguous(), n.contiguous()
-    ptrs = _pointers(len(pools))(*map(torch.Tensor.data_ptr, pools))
+    ptrs = array("Q", map(torch.Tensor.data_ptr, pools))
     rc = _call(index, _require_lib().cie_keep_path,
-               ptrs, len(pools), block_tables.data_ptr(), kv_lens.data_ptr(), path.data_ptr(),
+               ptrs.buffer_info()[0], len(pools), block_tables.data_ptr(), kv_lens.data_ptr(), path.data_ptr(),
                n.data_ptr(), new_lens.data_ptr(), B, T, shape[0], shape[1],
                block_tables.shape[1], shape[2] * shape[3] * 2)
     if rc:
