@@ -79,7 +79,7 @@ struct PagedParams {
   // tree mode on tcgen05 (tree_attn.cu)
   int pool_tokens;  // num_blocks * block_size: the maps' token extent
   int o_vec;        // o's rows are 16-byte aligned
-  int box_rows;     // tokens of a TMA box
+  int box_rows;     // tokens of a TMA box (8 or 16), 0: rows by cp.async
   int rg_rows;      // rows of a row group
   int min_run;      // fewest key tiles of a CTA
   int whole;        // tiles of the longest sequence up to which units are not cut

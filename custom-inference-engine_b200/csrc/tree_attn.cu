@@ -1,5 +1,5 @@
 // tree_attn.cu — attention of a tree of drafted tokens over the paged cache on
-// the tcgen05 tensor cores (head dims 64 and 128, pages of whole 8-token boxes).
+// the tcgen05 tensor cores (head dims 64 and 128).
 //
 // What it computes: see cie_tree_attn. The rows of a kv head (its G = Hq / Hkv
 // query heads times the T nodes) are packed into groups of up to 128, so that
@@ -7,8 +7,9 @@
 //   S = Q K^T            M = 128 rows, N = 64 keys, fp32 in TMEM
 //   P = 2^(S scale - m)  one thread per row (= TMEM lane), no shuffles
 //   O += P V             A = P from TMEM, fp32 in TMEM
-//   warp 0  TMA loader of K, warp 2 of V: one box of 8 or 16 tokens per page lookup,
-//           a lane each, into rings of 64-key tiles
+//   warp 0  loader of K, warp 2 of V, into rings of 64-key tiles: by TMA, one box of
+//           8 or 16 tokens per page lookup, a lane each, or, for pages that such boxes
+//           do not divide, by cp.async row by row
 //   warp 1  issues the MMAs, S two tiles ahead of PV in two TMEM buffers
 //   warps 4..7  softmax; a warp whose 32 rows are all padding does nothing
 // The history needs no mask. Only tiles that reach past it (the last T keys) are
@@ -205,7 +206,8 @@ __device__ __forceinline__ void store_f32x8(float* dst, const float (&x)[8]) {
                : "memory");
 }
 
-template <int D, bool BF16>
+// TMA = false: pages that no 8-token box divides; the loaders copy rows with cp.async.
+template <int D, bool BF16, bool TMA>
 __global__ void __launch_bounds__(kTcThreads, 2)
     tree_attn_kernel(const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v, const PagedParams p) {
@@ -282,61 +284,117 @@ __global__ void __launch_bounds__(kTcThreads, 2)
       uint64_t* full = is_k ? bar_k_full : bar_v_full;
       uint64_t* free_ = is_k ? bar_k_free : bar_v_free;
       constexpr int stages = C::ST;
-      const int per_slice = KEYS / p.box_rows;  // boxes along the tile's keys
-      const int box = lane % per_slice, slice = lane / per_slice;
-      if (lane == 0) tma_prefetch_desc(map);
-      // pool token of this lane's box of the unit's tile j; past the sequence, or for
-      // a refused page, a token outside the map, which TMA fills with zeros
-      auto coord = [&](int j) -> int {
-        const int t = j * KEYS + box * p.box_rows;
-        if (slice >= C::KCH || t >= w.kv_len) return p.pool_tokens;
+      const int32_t* tables = p.block_tables;
+      // pool token of position t of the piece's sequence, `none` past its end or for a
+      // refused page
+      auto token = [&](int t, int none) -> int {
+        if (t >= w.kv_len) return none;
         const int lb = p.bs_log2 >= 0 ? t >> p.bs_log2 : t / p.block_size;
-        const int blk = p.block_tables[static_cast<int64_t>(w.b) * p.max_blocks + lb];
+        const int blk = tables[static_cast<int64_t>(w.b) * p.max_blocks + lb];
         if (blk < 0 || blk >= p.num_blocks) {
           raise_status(CIE_DEV_BAD_BLOCK_ID);
-          return p.pool_tokens;
+          return none;
         }
         return blk * p.block_size + (p.bs_log2 >= 0 ? t & (p.block_size - 1) : t % p.block_size);
       };
-      int g = 0, j = 0, at = 0;
-      bool ok = true;
-      if (w.more) {
-        j = w.first;
-        at = coord(j);
-      }
-      while (ok && w.more) {
-        const int now = at;
-        const int st = g % stages;
-        // the next tile's lookup is in flight during the wait for a stage
-        auto look_up = [&]() {
-          if (++j == w.first + w.n) {
-            w.next(p, KEYS);
-            j = w.first;
-          }
-          if (w.more) at = coord(j);
-        };
-        if (g >= stages) look_up();
-        // the first Q goes ahead of all but the first K tile: behind the full rings of
-        // every SM its loads would wait for several microseconds
+      // wait for tile g's stage; the first Q goes ahead of all but the first K tile:
+      // behind the full rings of every SM its loads would wait for several microseconds
+      auto wait_stage = [&](int g) -> bool {
+        bool ok = true;
         if (g == (is_k ? 1 : 0))
           ok = __all_sync(0xffffffffu,
                           mbar_wait_bounded(bar_go, 0, abort_flag, &g_wait_limit_ns));
         if (ok && g >= stages)
-          ok = __all_sync(0xffffffffu, mbar_wait_bounded(free_ + st, (g / stages - 1) & 1,
-                                                         abort_flag, &g_wait_limit_ns));
-        if (!ok) break;
-        if (lane == 0) mbar_arrive_expect_tx(full + st, C::KV_BYTES);
-        __syncwarp();
-        if (slice < C::KCH)
-          tma_load_4d(ring + st * C::KV_BYTES + slice * KEYS * 128 + box * p.box_rows * 128, map,
-                      full + st, slice * 64, kvh, now, 0);
-        if (g < stages) look_up();
-        ++g;
-      }
-      if (*abort_flag && lane == 0) {
-        // copies still in flight land before the shared memory is released
-        for (int i = g - 1; i >= 0 && i >= g - stages; --i)
-          mbar_wait_timeout(full + i % stages, (i / stages) & 1, kWaitLimitNs);
+          ok = __all_sync(0xffffffffu,
+                          mbar_wait_bounded(free_ + g % stages, (g / stages - 1) & 1, abort_flag,
+                                            &g_wait_limit_ns));
+        return ok;
+      };
+      int g = 0, j = w.first;
+      auto advance = [&]() {  // to the run's next tile
+        if (++j == w.first + w.n) {
+          w.next(p, KEYS);
+          j = w.first;
+        }
+      };
+      if constexpr (TMA) {
+        const int per_slice = KEYS / p.box_rows;  // boxes along the tile's keys
+        const int box = lane % per_slice, slice = lane / per_slice;
+        if (lane == 0) tma_prefetch_desc(map);
+        // a token outside the map is filled with zeros
+        auto coord = [&]() {
+          return slice < C::KCH ? token(j * KEYS + box * p.box_rows, p.pool_tokens) : 0;
+        };
+        int at = w.more ? coord() : 0;
+        while (w.more) {
+          const int now = at, st = g % stages;
+          // the next tile's lookup is in flight during the wait for a stage
+          auto look_up = [&]() {
+            advance();
+            if (w.more) at = coord();
+          };
+          if (g >= stages) look_up();
+          if (!wait_stage(g)) break;
+          if (lane == 0) mbar_arrive_expect_tx(full + st, C::KV_BYTES);
+          __syncwarp();
+          if (slice < C::KCH)
+            tma_load_4d(ring + st * C::KV_BYTES + slice * KEYS * 128 + box * p.box_rows * 128, map,
+                        full + st, slice * 64, kvh, now, 0);
+          if (g < stages) look_up();
+          ++g;
+        }
+        if (*abort_flag && lane == 0) {
+          // copies still in flight land before the shared memory is released
+          for (int i = g - 1; i >= 0 && i >= g - stages; --i)
+            mbar_wait_timeout(full + i % stages, (i / stages) & 1, kWaitLimitNs);
+        }
+      } else {
+        constexpr int CPR = D / 8, RPI = 32 / CPR;  // 16-byte chunks of a row, rows at a time
+        const elem_t* pool = reinterpret_cast<const elem_t*>(is_k ? p.k_pool : p.v_pool) +
+                             kvh * D + (lane % CPR) * 8;
+        const int64_t tok_stride = static_cast<int64_t>(p.Hkv) * D;
+        const int ch = lane % CPR;
+        int row[2] = {-1, -1};  // pool tokens of the tile's keys lane and lane + 32
+        auto look_up = [&]() {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) row[h] = token(j * KEYS + h * 32 + lane, -1);
+        };
+        int told = 0;  // tiles announced to the MMA warp
+        auto announce = [&]() {  // the last tile copied is there: its waits are over
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(full + told % stages);
+          ++told;
+        };
+        if (w.more) look_up();
+        while (w.more) {
+          if (told < g && g >= stages &&
+              !__all_sync(0xffffffffu, mbar_test(free_ + g % stages, (g / stages - 1) & 1))) {
+            cp_async_wait<0>();
+            announce();
+          }
+          if (!wait_stage(g)) break;
+          uint8_t* dst = ring + (g % stages) * C::KV_BYTES + (ch / 8) * KEYS * 128;
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll 4
+            for (int i = 0; i < 32; i += RPI) {
+              const int r = i + lane / CPR, key = h * 32 + r;
+              const int tok = __shfl_sync(0xffffffffu, row[h], r);
+              cp_async_16(dst + key * 128 + (((ch % 8) ^ (key & 7)) * 16),
+                          pool + max(tok, 0) * tok_stride, tok >= 0);
+            }
+          cp_async_commit();
+          ++g;
+          advance();
+          if (w.more) look_up();
+          if (told < g - 1) {
+            cp_async_wait<1>();
+            announce();
+          }
+        }
+        cp_async_wait<0>();
+        if (told < g) announce();
       }
     } else if (warp == 1) {
       // ---------------------------------------------- MMA issuer (one elected lane)
@@ -874,16 +932,15 @@ struct TreePlan {
   int min_run, whole;
 };
 
-// The tcgen05 kernel takes head dims 64 and 128, pages of whole 8-token boxes and
-// trees whose bitmaps it holds (and lists and grids whose counts fit in an int), from
-// a single row on: even trees of 5 over 2.2 GB of K/V take 335 us there and 403 us in
+// The tcgen05 kernel takes head dims 64 and 128 and trees whose bitmaps it holds (and
+// lists and grids whose counts fit in an int), from a single row on: even trees of 5 over 2.2 GB of K/V take 335 us there and 403 us in
 // the mma.sync kernel, which serves everything else.
 static TreePlan tree_plan(int B, int Hq, int Hkv, int T, int d, int block_size, int max_blocks,
                           int split_tokens) {
   const int max_len = max_blocks * block_size;
   const int64_t R = static_cast<int64_t>(Hq / Hkv) * T;
   TreePlan tp{};
-  if ((d != 64 && d != 128) || block_size % 8 != 0 || T > kTcMaxTree ||
+  if ((d != 64 && d != 128) || T > kTcMaxTree ||
       static_cast<int64_t>(B) * (max_len / kTcKeys + 1 + kTcOpen) >= (1 << 30) ||
       static_cast<int64_t>(Hkv) * ((R + 127) / 128) > 4096) {
     tp.pl = make_plan(B, Hq, Hkv, T, d, max_len, split_tokens);
@@ -920,11 +977,11 @@ static TreePlan tree_plan(int B, int Hq, int Hkv, int T, int d, int block_size, 
   return tp;
 }
 
-template <int D, bool BF16>
+template <int D, bool BF16, bool TMA>
 static int launch_tree_tc(const CUtensorMap& mk, const CUtensorMap& mv, const PagedParams& prm,
                           const TreePlan& tp, cudaStream_t st) {
   constexpr int smem = TcCfg<D>::SMEM;
-  auto kern = tree_attn_kernel<D, BF16>;
+  auto kern = tree_attn_kernel<D, BF16, TMA>;
   cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   kern<<<tp.ctas, kTcThreads, smem, st>>>(mk, mv, prm);
   CIE_CHECK_LAUNCH("tree_attn_kernel");
@@ -953,19 +1010,20 @@ static int launch_tree_tc(const CUtensorMap& mk, const CUtensorMap& mv, const Pa
 
 template <int D, bool BF16>
 static int dispatch_tree_tc(const PagedParams& prm, const TreePlan& tp, cudaStream_t st) {
+  CUtensorMap mk{}, mv{};
+  if (prm.box_rows == 0) return launch_tree_tc<D, BF16, false>(mk, mv, prm, tp, st);
   // (d, head, pool token, 1) with a (64, 1, 8 or 16, 1) box, 128-byte swizzle
   const cuuint64_t tokens = static_cast<cuuint64_t>(prm.pool_tokens);
   const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)prm.Hkv, tokens, 1};
   const cuuint64_t strides[3] = {(cuuint64_t)D * 2, (cuuint64_t)prm.Hkv * D * 2,
                                  tokens * prm.Hkv * D * 2};
   const cuuint32_t box[4] = {64, 1, (cuuint32_t)prm.box_rows, 1};
-  CUtensorMap mk, mv;
   if (!make_kv_map(&mk, prm.k_pool, D, dims, strides, box, BF16) ||
       !make_kv_map(&mv, prm.v_pool, D, dims, strides, box, BF16)) {
     set_error("cie_tree_attn: cuTensorMapEncodeTiled failed for the pools");
     return CIE_ERR_LAUNCH;
   }
-  return launch_tree_tc<D, BF16>(mk, mv, prm, tp, st);
+  return launch_tree_tc<D, BF16, true>(mk, mv, prm, tp, st);
 }
 
 }  // namespace cie
@@ -1050,7 +1108,7 @@ extern "C" int cie_tree_attn(const void* q, const void* k_pool, const void* v_po
   prm.pool_tokens = num_blocks * block_size;
   prm.o_vec = aligned16(o) && o_strides[0] % 8 == 0 && o_strides[1] % 8 == 0 &&
               o_strides[2] % 8 == 0;
-  prm.box_rows = block_size % 16 == 0 ? 16 : 8;
+  prm.box_rows = block_size % 16 == 0 ? 16 : block_size % 8 == 0 ? 8 : 0;
   prm.rg_rows = pl.rg_rows;
   prm.min_run = tp.min_run;
   prm.whole = tp.whole;

@@ -105,6 +105,9 @@ ATTN = [
     (1, 1024, 1, 1, 32, 16, FP16, [1024], "chain"),
     (2, 9, 4, 2, 64, 5, BF16, [23, 61], "roots"),
     (3, 6, 5, 1, 128, 16, BF16, [2500, 6, 33], "star"),
+    (3, 18, 8, 2, 128, 20, FP16, [18, 700, 1999], "random"),
+    (2, 40, 8, 4, 64, 12, BF16, [1234, 2500], "binary"),
+    (2, 7, 4, 4, 128, 1, BF16, [90, 400], "random"),
 ]
 
 
@@ -114,7 +117,7 @@ def test_tree_attention(B, T, Hq, Hkv, D, bs, dtype, lens, kind):
 
 
 @pytest.mark.parametrize("split", [16, 48, 256])
-@pytest.mark.parametrize("B,T,Hq,Hkv,D,bs,dtype,lens,kind", [ATTN[4], ATTN[5], ATTN[12], ATTN[10], ATTN[14]])
+@pytest.mark.parametrize("B,T,Hq,Hkv,D,bs,dtype,lens,kind", [ATTN[4], ATTN[5], ATTN[12], ATTN[10], ATTN[14], ATTN[22]])
 def test_tree_attention_partitions(B, T, Hq, Hkv, D, bs, dtype, lens, kind, split):
     check(setup(B, T, Hq, Hkv, D, bs, dtype, lens, kind, seed=3), split_tokens=split)
 
@@ -130,12 +133,12 @@ def test_tree_attention_shared_tree():
     check(s)
 
 
-@pytest.mark.parametrize("D,T,Hq", [(128, 32, 32), (64, 12, 32), (64, 48, 32), (128, 40, 64)])
-def test_tree_attention_many_units(D, T, Hq):
+@pytest.mark.parametrize("D,T,Hq,bs", [(128, 32, 32, 16), (64, 12, 32, 16), (64, 48, 32, 24), (128, 40, 64, 16), (128, 20, 32, 20), (64, 6, 32, 10)])
+def test_tree_attention_many_units(D, T, Hq, bs):
     """More work than fits on the GPU at once, in ragged sequences: every pipeline wait ends (the
     status word stays clear) and repeated calls agree bit for bit."""
     rs = np.random.RandomState(D + T)
-    s = setup(32, T, Hq, 8, D, 16, BF16, [int(x) for x in rs.randint(T, 6000, 32)], seed=21)
+    s = setup(32, T, Hq, 8, D, bs, BF16, [int(x) for x in rs.randint(T, 6000, 32)], seed=21)
     out = run(s)
     for _ in range(10):
         assert torch.equal(run(s), out)
@@ -217,7 +220,7 @@ def test_tree_attention_bad_parents_are_roots(cuda):
     assert torch.equal(out, run(s))
 
 
-@pytest.mark.parametrize("D,T,bs", [(64, 6, 16), (128, 40, 16), (64, 6, 12)])
+@pytest.mark.parametrize("D,T,bs", [(64, 6, 16), (128, 40, 16), (64, 6, 12), (128, 6, 24), (32, 6, 12)])
 def test_tree_attention_bad_block_id(cuda, D, T, bs):
     from kernels import _lib
 
