@@ -272,6 +272,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  int copies = 0;  // loader warps: TMA tiles issued
 
   if (warp < 4) {
     TcWalk w;
@@ -341,12 +342,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
             tma_load_4d(ring + st * C::KV_BYTES + slice * KEYS * 128 + box * p.box_rows * 128, map,
                         full + st, slice * 64, kvh, now, 0);
           if (g < stages) look_up();
-          ++g;
-        }
-        if (*abort_flag && lane == 0) {
-          // copies still in flight land before the shared memory is released
-          for (int i = g - 1; i >= 0 && i >= g - stages; --i)
-            mbar_wait_timeout(full + i % stages, (i / stages) & 1, kWaitLimitNs);
+          copies = ++g;
         }
       } else {
         constexpr int CPR = D / 8, RPI = 32 / CPR;  // 16-byte chunks of a row, rows at a time
@@ -842,6 +838,12 @@ __global__ void __launch_bounds__(kTcThreads, 2)
   __syncthreads();
   tc_fence_after();
   if (warp == 1) tmem_dealloc(tmem, C::TM_COLS);
+  // a role gave up: copies still in flight land before the shared memory is released
+  if (*abort_flag && copies > 0 && lane == 0) {
+    uint64_t* full = warp == 0 ? bar_k_full : bar_v_full;
+    for (int i = copies - 1; i >= 0 && i >= copies - C::ST; --i)
+      mbar_wait_timeout(full + i % C::ST, (i / C::ST) & 1, kWaitLimitNs);
+  }
 }
 
 // Joins the partial results of the units that the runs' borders cut: piece i of a

@@ -266,6 +266,29 @@ def test_tree_attention_graph_and_streams(D, T, Hq):
     assert_within(o1, ref, bound)
 
 
+@pytest.mark.parametrize("D,bs,T", [(128, 16, 8), (64, 20, 30), (32, 16, 8)])
+def test_tree_attention_wait_that_runs_out(cuda, D, bs, T):
+    """With a wait limit of 0 the kernels give up at the first wait that is not over at once, say so in
+    the status word and leave the context usable. (At d = 32 the tiles, out of L2, may all be there in
+    time: then no wait ran out, and the output is the right one.)"""
+    from kernels import _lib
+
+    rs = np.random.RandomState(22)
+    s = setup(16, T, 16, 4, D, bs, BF16, [int(x) for x in rs.randint(3000, 6000, 16)], seed=22)
+    want = run(s)
+    torch.cuda.synchronize()
+    old = _lib.set_wait_limit(0)
+    try:
+        out = run(s)
+        torch.cuda.synchronize()
+    finally:
+        _lib.set_wait_limit(old)
+    status = _lib.device_status()
+    assert status == _lib.CIE_DEV_TIMEOUT or (D == 32 and status == 0 and torch.equal(out, want))
+    for _ in range(3):
+        assert torch.equal(run(s), want)
+
+
 # ------------------------------------------------------------------ append
 @pytest.mark.parametrize("D,Hkv,dtype", [(64, 2, BF16), (128, 8, FP16), (16, 1, BF16)])
 def test_rope_append_of_a_tree(D, Hkv, dtype):
