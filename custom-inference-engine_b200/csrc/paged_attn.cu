@@ -33,7 +33,11 @@
 // Each CTA reads the M parent indices once and turns them into one ancestor
 // bitmap per row (RG x ceil(M / 32) words in shared memory), so only the tiles
 // that reach past the history pay for the mask: a 16-bit window per row and
-// tile. Everything before them is the unmasked loop of the decode kernel.
+// tile. Everything before them is the unmasked loop of the decode kernel. It serves
+// the head dims and tree sizes that tree_attn.cu does not (d 16, 32 and 256, more
+// than 256 nodes); more than 32 rows per kv head (64 at d <= 64) read K/V again for
+// every group of rows: 776 us for trees of 16 over 2.2 GB of K/V at d = 128, where
+// the tcgen05 kernel takes 350.
 #include <cuda.h>
 #include <cuda_runtime.h>
 

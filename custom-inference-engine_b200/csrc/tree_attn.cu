@@ -35,6 +35,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <cfloat>
 #include <cstdint>
 #include <type_traits>
 
@@ -466,10 +467,17 @@ __global__ void __launch_bounds__(kTcThreads, 2)
         for (int b = lane; b < p.B; b += 32)
           if (p.kv_lens[b] > p.max_blocks * p.block_size) raise_status(CIE_DEV_BAD_BLOCK_ID);
       for (int b = blockIdx.x; b < p.B; b += gridDim.x)
-        if (tc_len(p, b) == 0)  // an empty sequence: zeros
-          for (int i = lane; i < p.Hq * p.M * D; i += 32)
-            reinterpret_cast<elem_t*>(p.o)[b * p.o_sb + (i / (p.M * D)) * p.o_sh +
-                                           (i / D % p.M) * p.o_sm + i % D] = elem_t(0.f);
+        if (tc_len(p, b) == 0)  // an empty sequence: zeros, 8 elements at a time
+          for (int i = lane; i < p.Hq * p.M * (D / 8); i += 32) {
+            const int r = i / (D / 8);
+            elem_t* o = reinterpret_cast<elem_t*>(p.o) + b * p.o_sb + (r / p.M) * p.o_sh +
+                        (r % p.M) * p.o_sm + (i % (D / 8)) * 8;
+            if (p.o_vec) {
+              *reinterpret_cast<uint4*>(o) = make_uint4(0, 0, 0, 0);
+            } else {
+              for (int e = 0; e < 8; ++e) o[e] = elem_t(0.f);
+            }
+          }
     }
   } else {
     if (warp - 4 < active) {
@@ -1035,7 +1043,8 @@ using namespace cie;
 extern "C" size_t cie_tree_attn_workspace(int B, int Hq, int Hkv, int T, int d, int block_size,
                                           int max_blocks, int split_tokens) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || T <= 0 || Hq % Hkv != 0 || !mma_head_dim_ok(d) ||
-      block_size <= 0 || max_blocks < 0)
+      block_size <= 0 || max_blocks < 0 ||
+      static_cast<int64_t>(max_blocks) * block_size >= (int64_t(1) << 31) - 4096)
     return 0;
   return tree_plan(B, Hq, Hkv, T, d, block_size, max_blocks, split_tokens).pl.workspace();
 }
@@ -1061,6 +1070,8 @@ extern "C" int cie_tree_attn(const void* q, const void* k_pool, const void* v_po
   CIE_CHECK_ARG(static_cast<int64_t>(max_blocks) * block_size < (int64_t(1) << 31) - 4096,
                 "cie_tree_attn: max_blocks * block_size too large");
   CIE_CHECK_ARG(q_strides && o_strides, "cie_tree_attn: null strides");
+  // the kernels take the largest score for the largest exponent
+  CIE_CHECK_ARG(scale > 0.f && scale <= FLT_MAX, "cie_tree_attn: scale must be positive and finite");
   CIE_CHECK_ARG(aligned16(q) && aligned16(k_pool) && aligned16(v_pool),
                 "cie_tree_attn: q/k_pool/v_pool must be 16-byte aligned");
   CIE_CHECK_ARG(q_strides[0] % 8 == 0 && q_strides[1] % 8 == 0 && q_strides[2] % 8 == 0,

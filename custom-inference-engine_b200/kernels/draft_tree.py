@@ -14,7 +14,7 @@ tree, a batch of trees is served at once, and nothing waits for the host:
 A tree is an int32 tensor ``parents``, (T,) for one tree shared by the batch or
 (B, T): parents[i] < i is node i's parent, -1 none. Node 0 is the root, the last
 token that is already decided; a chain is ``[-1, 0, 1, ..]``. Smaller trees of a
-batch are padded with nodes of parent -1, which belong to no path. The nodes sit
+batch are padded with nodes of parent -1 (and any token), which belong to no path. The nodes sit
 in the last T slots of their sequence, written by
 ``kernels.flash_attention.rope_append(..., parents=parents)``.
 
@@ -120,7 +120,7 @@ def tree_attention(
     before them, itself and its ancestors by ``parents``. ``rope`` rotates its q at
     position kv_lens[b] - T + depth. Returns (B, Hq, T, D) in q's dtype; zeros for
     kv_lens[b] = 0. NaN or infinity in a node's K or V reaches only the nodes that
-    see it.
+    see it. ``scale`` must be positive (default 1 / sqrt(D)).
     """
     index = q.get_device()
     if index < 0:

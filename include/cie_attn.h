@@ -259,7 +259,9 @@ int cie_rope_append_tree(const void* k_new, const void* v_new, void* k_pool,
  * the K or V row of a node reaches only the rows that see it. A sequence with
  * kv_lens[b] = 0 gives zeros; a node whose slot would lie before the first
  * (0 < kv_lens[b] < T) sees no key and gives NaN. Bad parents: as above.
- * T <= CIE_MAX_TREE.
+ * scale must be positive. split_tokens: 0 = automatic (the split follows the
+ * lengths on the device); else tokens of a partition, rounded up to 64 by the
+ * tcgen05 kernel. T <= CIE_MAX_TREE.
  */
 int cie_tree_attn(const void* q, const void* k_pool, const void* v_pool,
                   const int32_t* block_tables, const int32_t* kv_lens,
@@ -303,7 +305,7 @@ size_t cie_tree_attn_workspace(int B, int Hq, int Hkv, int T, int d,
  *               token, then -1
  * A target row without a finite positive sum gives the last token -1 and sets
  * CIE_DEV_BAD_PROBS; a drafted token outside [0, V) is never kept and sets
- * CIE_DEV_BAD_TREE. Outputs contiguous. T <= CIE_MAX_TREE, V <= 2^23.
+ * CIE_DEV_BAD_TREE (a node without a parent may hold any token). Outputs contiguous. T <= CIE_MAX_TREE, V <= 2^23.
  */
 int cie_verify_drafts(const void* tokens, int64_t tokens_stride_b,
                       int tokens_64bit, const int32_t* parents,

@@ -52,6 +52,8 @@ def test_tree_attention_refuses(lib):
     refused(f(*tree_args(qs=(ctypes.c_int64 * 3)(64, 64, 60))), "multiples of 8")
     refused(f(*tree_args(k=ctypes.c_void_p(4104))), "aligned")
     refused(f(*tree_args(split=24)), "multiple of 16")
+    for scale in (0.0, -0.5, float("nan"), float("inf")):
+        refused(f(*tree_args(scale=scale)), "positive")
     refused(f(*tree_args(cos=P)), "both")
     refused(f(*tree_args(cos=P, sin=P)), "rope_max_pos")
     refused(f(*tree_args(psb=-1)), "stride")
@@ -61,6 +63,7 @@ def test_tree_attention_refuses(lib):
     assert lib.cie_tree_attn_workspace(1, 4, 2, 5, 64, 16, 4096, 0) > 0
     assert lib.cie_tree_attn_workspace(1, 4, 2, 5, 64, 16, 4, 0) == 0
     assert lib.cie_tree_attn_workspace(1, 4, 3, 5, 64, 16, 4, 0) == 0
+    assert lib.cie_tree_attn_workspace(1, 4, 2, 5, 64, 16, 1 << 28, 0) == 0
 
 
 def test_rope_append_tree_refuses(lib):

@@ -147,6 +147,60 @@ def test_tree_attention_many_units(D, T, Hq, bs):
     assert_within(out[pick], ref, bound)
 
 
+@pytest.mark.parametrize("B,T,Hq,Hkv,D,bs,lens", [
+    (700, 3, 4, 2, 64, 16, lambda rs: [int(x) * int(y) for x, y in zip(rs.randint(3, 90, 700), rs.rand(700) > 0.3)]),  # many, a third idle
+    (300, 4, 4, 4, 128, 8, lambda rs: [2500] + [int(x) for x in rs.randint(0, 60, 298)] + [1900]),                     # two long among short
+    (3, 40, 320, 40, 64, 16, lambda rs: [700, 41, 40]),                                                               # more head groups than CTAs for one part each
+    (1, 50, 256, 1, 128, 16, lambda rs: [1500]),                                                                      # a hundred row groups
+])
+def test_tree_attention_batches(B, T, Hq, Hkv, D, bs, lens):
+    rs = np.random.RandomState(B)
+    s = setup(B, T, Hq, Hkv, D, bs, BF16, lens(rs), "random", seed=B)
+    out = run(s)
+    pick = sorted(set([0, B - 1] + [int(x) for x in rs.randint(0, B, 40)]))
+    ref, bound = tree_attention_ref(s["q"][pick], s["k"], s["v"], s["tables"][pick], s["lens"][pick], s["parents"][pick])
+    assert_within(out[pick], ref, bound)
+    idle = [b for b in range(B) if int(s["lens"][b]) == 0]
+    assert not idle or float(out[idle].abs().max()) == 0.0
+
+
+def test_tree_attention_length_beyond_the_table(cuda):
+    """A length that the table cannot hold is reported and cut to what it holds."""
+    from kernels import _lib
+
+    for D, T in ((128, 6), (32, 6)):
+        s = setup(2, T, 8, 2, D, 16, BF16, [128, 100], seed=23)
+        s["k"].nan_to_num_(0)
+        s["v"].nan_to_num_(0)
+        want = run(s)
+        s["lens"][0] = 5000
+        out = run(s)
+        assert _lib.device_status() == _lib.CIE_DEV_BAD_BLOCK_ID
+        assert torch.equal(out, want)
+
+
+def test_pools_beyond_32_bits():
+    """Pages behind the first 4 GB of a pool: attention, append and the kept path."""
+    from kernels.draft_tree import keep_path
+    from kernels.flash_attention import rope_append
+
+    D, Hkv, T, nb = 128, 8, 7, 140_000                       # 4.6 GB a pool
+    s = setup(2, T, 16, Hkv, D, 16, BF16, [300, 90], seed=24)
+    big = dict(s, k=torch.empty(nb, 16, Hkv, D, dtype=BF16, device="cuda"), v=torch.empty(nb, 16, Hkv, D, dtype=BF16, device="cuda"))
+    n = s["k"].shape[0]
+    big["k"][nb - n:], big["v"][nb - n:] = s["k"], s["v"]
+    big["tables"] = s["tables"] + (nb - n)
+    assert torch.equal(run(big), run(s))
+    kn, vn = torch.randn(2, T, Hkv, D, device="cuda").to(BF16), torch.randn(2, T, Hkv, D, device="cuda").to(BF16)
+    path = torch.tensor([[0, 2, 5, -1, -1, -1, -1], [0, 1, 3, 6, -1, -1, -1]], dtype=torch.int32, device="cuda")
+    kept = torch.tensor([3, 4], dtype=torch.int32, device="cuda")
+    for x in (s, big):
+        rope_append(kn, vn, x["k"], x["v"], x["tables"], x["lens"] - T, rope=rope_tables(D), parents=x["parents"])
+        keep_path([x["k"], x["v"]], x["tables"], x["lens"], path, kept)
+    for name in "kv":
+        assert torch.equal(big[name][nb - n:].view(torch.int16), s[name].view(torch.int16))
+
+
 @pytest.mark.parametrize("D,Hq,Hkv,T", [(64, 8, 2, 6), (128, 8, 2, 40), (32, 4, 4, 6)])
 def test_tree_attention_idle_and_short_sequences(D, Hq, Hkv, T):
     """A sequence of length 0 gives zeros; one shorter than the tree has no slots for its first nodes."""
@@ -448,6 +502,17 @@ def test_verify_bad_rows_and_tokens(cuda):
             assert _lib.device_status() == _lib.CIE_DEV_BAD_TREE
             assert [g.tolist() for g in got] == list(verify_ref(t, parents, p, kw.get("uniforms"), kw.get("draft_probs")))
             assert got.n[0].item() == 1
+
+
+def test_verify_padded_trees():
+    """Nodes without a parent fill a batch's smaller trees; their tokens may be anything."""
+    parents = torch.tensor([[-1, 0, 0, 1], [-1, 0, -1, -1], [-1, -1, -1, -1]], dtype=torch.int32, device="cuda")
+    p, q, u = probs(3, 4, 900, 16)
+    tokens = drafted(q, parents, 17)
+    tokens[1, 2:], tokens[2] = -1, -1
+    for kw in (dict(uniforms=u, draft=q), dict(uniforms=u), dict()):
+        got = check_verify(tokens, parents, p, **kw)
+        assert got.n[2].item() == 1 and got.n[1].item() <= 2
 
 
 def test_verify_greedy_ties_and_nan():
