@@ -49,13 +49,14 @@ constexpr int kTcKeys = 64;      // keys of a tile
 constexpr int kTcBufs = 2;       // S buffers
 constexpr int kTcThreads = 256;
 // Tiles of the longest sequence up to which sequences stay whole: cutting 16 tiles
-// of one sequence in four and joining them took 17 us, leaving them whole 21 us.
+// of one sequence in four and joining them takes 14 us, leaving them whole 21 us.
 constexpr int kTcWhole = 8;
-// Shortest run of tiles worth a CTA of its own, and the tiles that opening and
-// closing a piece costs. With 8 and 2 instead of 4 and 4 a ragged fp16 batch
-// (12 contexts of up to 8K, trees of 27, d = 64) took 51 against 48 us.
+// Shortest run of tiles worth a CTA of its own (with 6 instead of 4 one context of 1K
+// took 20 against 17 us), and the tiles that one more piece costs a CTA (trees of 24
+// over 4 contexts of up to 4K, 16 heads: 32, 29, 26 and 25 us with 4, 5, 8 and 12;
+// trees of 12 over 64 contexts of up to 8K, d = 64: 133 us with 8, 136 with 12).
 constexpr int kTcMinRun = 4;
-constexpr int kTcOpen = 4;
+constexpr int kTcOpen = 8;
 
 template <int D>
 struct TcCfg {
@@ -76,8 +77,8 @@ struct TcCfg {
 // ------------------------------------------------------------------ work split
 // CTA c works for head group c % groups (groups = kv heads * row groups) and takes
 // part c / groups of that group's list: the key tiles of all sequences end to end,
-// each sequence behind kTcOpen idle places that stand for what opening and closing
-// a piece costs. The CTAs of one part thus read the same token rows, one head each,
+// with kTcOpen idle places between two sequences that stand for what one more piece
+// costs a CTA. The CTAs of one part thus read the same token rows, one head each,
 // at about the same time: at d = 64 two heads share a 256-byte fetch, and lists that
 // ran through the heads one after the other took twice as long.
 __device__ __forceinline__ int tc_len(const PagedParams& p, int b) {
@@ -106,7 +107,7 @@ __device__ __forceinline__ TcPlan tc_plan(const PagedParams& p, int keys, int pa
   sum = __reduce_add_sync(0xffffffffu, sum);
   most = __reduce_max_sync(0xffffffffu, most);
   TcPlan plan;
-  plan.run = max((sum + parts - 1) / parts, p.min_run + kTcOpen);
+  plan.run = max((sum - kTcOpen + parts - 1) / parts, p.min_run);
   plan.whole = most <= p.whole;
   return plan;
 }
@@ -160,7 +161,7 @@ struct TcWalk {
       deal(p, keys);
       return;
     }
-    lo = part * plan.run;
+    lo = part * plan.run + kTcOpen;  // the list begins with a tile: every CTA opens one piece
     hi = lo + plan.run;
     at = 0;
     b = 0;
@@ -873,7 +874,7 @@ __global__ void __launch_bounds__(kTcMergeThreads)
   int at = 0;  // the sequence's place in the list
   if (lane < b) at = mine;
   for (int i = lane + 32; i < b; i += 32) at += tc_places((tc_len(p, i) + keys - 1) / keys);
-  at = __reduce_add_sync(0xffffffffu, at) + kTcOpen;
+  at = __reduce_add_sync(0xffffffffu, at);
   const int c0 = at / plan.run, c1 = (at + tiles - 1) / plan.run;  // parts that share it
   // The partial results are there. Every CTA waits, also one without work: what
   // follows this kernel on the stream may count on the whole call being done.
