@@ -737,3 +737,37 @@ def test_tree_step_has_no_host_sync_before_its_end():
     finally:
         torch.cuda.set_sync_debug_mode("default")
     assert lens.tolist() == [6 + n for n in v.n.tolist()]
+
+
+def test_two_streams_at_once():
+    """Calls that overlap on two streams share nothing: each gives what it gives alone."""
+    from kernels.draft_tree import keep_path, tree_attention, verify_drafts
+
+    sets = []
+    for i, (D, T) in enumerate(((128, 20), (64, 9))):
+        s = setup(6, T, 16, 4, D, 16, BF16, [T + 300 * b for b in range(6)], seed=30 + i)
+        p, q, u = probs(6, T, 20000 + i, 31 + i)
+        tokens = drafted(q, s["parents"], 32 + i)
+        pool = torch.randn(s["k"].shape, device="cuda").to(BF16)
+        sets.append((s, (tokens, s["parents"], p, u, q), pool))
+
+    def one(x):
+        s, v, pool = x
+        out = tree_attention(s["q"], s["k"], s["v"], s["tables"], s["lens"], s["parents"])
+        verdict = verify_drafts(*v)
+        moved = pool.clone()
+        lens = keep_path([moved], s["tables"], s["lens"], verdict.path, verdict.n)
+        return [out, *verdict, moved, lens]
+
+    want = [one(x) for x in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for k, x in enumerate(sets):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(one(x))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for r in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(r, want[k]))
