@@ -37,7 +37,8 @@
 // the head dims and tree sizes that tree_attn.cu does not (d 16, 32 and 256, more
 // than 256 nodes); more than 32 rows per kv head (64 at d <= 64) read K/V again for
 // every group of rows: 776 us for trees of 16 over 2.2 GB of K/V at d = 128, where
-// the tcgen05 kernel takes 350.
+// the tcgen05 kernel took 350 (P rounded once in both). P in two halves: 73 against 69 us
+// for 16 rows at d = 256, 436 against 400 us for 256 rows at d = 32.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -529,8 +530,9 @@ __global__ void __launch_bounds__(kPagedWarps * 32)
     // reference to within one fp16 rounding (the reference's own fp16 kernel
     // test asks for 1e-3 where outputs reach |2|, i.e. half an ulp). bf16 keeps a
     // single rounding: its output ulp (2^-8) dwarfs the P error, and the second
-    // PV MMA measured 10% slower on the verify workload.
-    constexpr bool kSplitP = !BF16;
+    // PV MMA measured 10% slower on the verify workload. Tree mode holds P in two
+    // halves for both types, as tree_attn.cu does and for its reason.
+    constexpr bool kSplitP = !BF16 || TREE;
     uint32_t pa[MT][4];
     uint32_t pl[kSplitP ? MT : 1][4];
     float alpha[MT][2];
@@ -574,13 +576,12 @@ __global__ void __launch_bounds__(kPagedWarps * 32)
         }
         l_run[mt][hf] = l_run[mt][hf] * alpha[mt][hf] + ps;
         // A fragment of P: a0/a1 = rows g/g+8, tokens 2t..2t+1; a2/a3 = tokens 8+2t..
-        pa[mt][hf] = pack2<BF16>(v[0], v[1]);
-        pa[mt][2 + hf] = pack2<BF16>(v[2], v[3]);
         if constexpr (kSplitP) {
-          const float2 h01 = unpack2<BF16>(pa[mt][hf]);
-          const float2 h23 = unpack2<BF16>(pa[mt][2 + hf]);
-          pl[mt][hf] = pack2<BF16>(v[0] - h01.x, v[1] - h01.y);
-          pl[mt][2 + hf] = pack2<BF16>(v[2] - h23.x, v[3] - h23.y);
+          split2<BF16>(v[0], v[1], pa[mt][hf], pl[mt][hf]);
+          split2<BF16>(v[2], v[3], pa[mt][2 + hf], pl[mt][2 + hf]);
+        } else {
+          pa[mt][hf] = pack2<BF16>(v[0], v[1]);
+          pa[mt][2 + hf] = pack2<BF16>(v[2], v[3]);
         }
       }
     }

@@ -448,4 +448,23 @@ __device__ __forceinline__ float2 unpack2(uint32_t u) {
   }
 }
 
+// Two values as hi + lo of 16 bits each. fp16: hi rounded, 2^-22 relative in all.
+// bf16: hi is the upper half of the fp32 value (one byte permute for the pair, off by
+// less than 2^-7, and the rest is exact), lo is rounded: 2^-15 relative in all.
+template <bool BF16>
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  float2 h;
+  if constexpr (BF16) {
+    const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+    hi = __byte_perm(a, b, 0x7632);
+    h = make_float2(__uint_as_float(a & 0xffff0000u), __uint_as_float(b & 0xffff0000u));
+  } else {
+    hi = pack2<BF16>(x, y);
+    h = unpack2<BF16>(hi);
+  }
+  float l0, l1;
+  f2_unpack(fadd2(f2_pack(x, y), f2_pack(-h.x, -h.y)), l0, l1);
+  lo = pack2<BF16>(l0, l1);
+}
+
 }  // namespace cie

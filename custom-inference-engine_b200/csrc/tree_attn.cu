@@ -6,7 +6,7 @@
 // every K and V byte is read once for all rows of a group:
 //   S = Q K^T            M = 128 rows, N = 64 keys, fp32 in TMEM
 //   P = 2^(S scale - m)  one thread per row (= TMEM lane), no shuffles
-//   O += P V             A = P from TMEM, fp32 in TMEM
+//   O += P V             A = P from TMEM as two halves of 16 bits, fp32 in TMEM
 //   warp 0  loader of K, warp 2 of V, into rings of 64-key tiles: by TMA, one box of
 //           8 or 16 tokens per page lookup, a lane each, or, for pages that such boxes
 //           do not divide, by cp.async row by row
@@ -24,14 +24,23 @@
 // contexts of up to 8K at d = 64.) Batches of short sequences are dealt out whole
 // and need no merge.
 //
+// Precision: scores, the softmax's maximum and sum, O and the merge are fp32. P goes
+// to the tensor cores as hi + lo (2^-15 relative in bf16, 2^-22 in fp16), so that of
+// the roundings to 16 bits only the output's own is left, and q's behind its rotation,
+// where the model rounds it too. Rounded once to bf16 P costs the output as much again
+// as its own rounding (2.3e-3 against 1.7e-3 off in the 2-norm).
+//
 // Bound: K/V bytes. A 64-key tile is 32 KB at d = 128, about 1400 cycles of one
-// SM's share of HBM; its MMAs take 640 and its exponentials 512 cycles (MUFU). Two
+// SM's share of HBM; its MMAs take 960 and its exponentials 512 cycles (MUFU). Two
 // CTAs share an SM (256 TMEM columns, ~100 KB each), so one's hand-offs hide behind
-// the other's. More than 128 rows take another pass over K/V, which comes from L2:
-// 99 us for trees of 64 over 8 contexts of up to 16K (256 rows), against 103 us for
-// a form with two 128-row tiles in one CTA that fills the SM by itself.
-// Measured on B200 (2.2 GB of K/V, 32 contexts of 1K-32K, d = 128): trees of 5
-// 335 us (6.6 TB/s), of 16 352 us (6.3 TB/s), of 32 383 us (5.8 TB/s).
+// the other's. More than 128 rows take another pass over K/V, which comes from L2.
+// Measured on B200 (2.2 GB of K/V, 32 contexts of 1K-32K, d = 128, bf16): trees of 5
+// 340 us (6.5 TB/s), of 16 371 us (6.0 TB/s), of 32 422 us (5.3 TB/s); with P rounded
+// once 328, 346 and 375 us. Trees of 64 over 8 contexts of up to 16K (256 rows) 112 us,
+// with P rounded once 98; so measured, a form with two 128-row tiles in one CTA that
+// fills the SM by itself took 103.
+//
+// The choices below were measured with P rounded once to bf16.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -215,8 +224,6 @@ __global__ void __launch_bounds__(kTcThreads, 2)
                      const __grid_constant__ CUtensorMap tm_v, const PagedParams p) {
   using C = TcCfg<D>;
   constexpr int KEYS = kTcKeys, NBUF = kTcBufs;
-  // fp16: P as two halves (p_hi + p_lo), as in paged_attn.cu and for its reason
-  constexpr bool kSplitP = !BF16;
   using elem_t = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -443,7 +450,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
           const uint32_t acc0 = j > 0 || (w.first + 1) * KEYS > hist ? 1u : 0u;
           const uint32_t p_col = tmem + (g % NBUF) * KEYS;
 #pragma unroll
-          for (int half = 0; half < (kSplitP ? 2 : 1); ++half)
+          for (int half = 0; half < 2; ++half)  // P's upper and lower halves
 #pragma unroll
             for (int kk = 0; kk < KEYS / 16; ++kk)
               if (elect_one_sync())
@@ -746,13 +753,13 @@ __global__ void __launch_bounds__(kTcThreads, 2)
             fence_proxy_async_smem();
           }
 
-          // p = 2^(s * scale - m) in groups of 8 pairs, packed to 16 bits
+          // p = 2^(s * scale - m) in groups of 8 pairs, as two halves of 16 bits
           const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2);
           const uint64_t nm2 = f2_pack(-m_use, -m_use);
           uint64_t sum_a = f2_pack(0.f, 0.f), sum_b = sum_a;
 #pragma unroll
           for (int h = 0; h < KEYS / 32; ++h) {  // 32 keys = 16 columns of P
-            uint32_t pk[16], pl[kSplitP ? 16 : 1];
+            uint32_t pk[16], pl[16];
 #pragma unroll
             for (int g0 = 0; g0 < 16; g0 += 8) {
               float e[16];
@@ -768,15 +775,11 @@ __global__ void __launch_bounds__(kTcThreads, 2)
                 const uint64_t p2 = f2_pack(e[2 * i], e[2 * i + 1]);
                 if (i & 1) sum_b = fadd2(sum_b, p2);
                 else sum_a = fadd2(sum_a, p2);
-                pk[g0 + i] = pack2<BF16>(e[2 * i], e[2 * i + 1]);
-                if constexpr (kSplitP) {
-                  const float2 hi = unpack2<BF16>(pk[g0 + i]);
-                  pl[g0 + i] = pack2<BF16>(e[2 * i] - hi.x, e[2 * i + 1] - hi.y);
-                }
+                split2<BF16>(e[2 * i], e[2 * i + 1], pk[g0 + i], pl[g0 + i]);
               }
             }
             tmem_st16(s_col + h * 16, pk);
-            if constexpr (kSplitP) tmem_st16(s_col + KEYS / 2 + h * 16, pl);
+            tmem_st16(s_col + KEYS / 2 + h * 16, pl);
           }
           float s0, s1;
           f2_unpack(fadd2(sum_a, sum_b), s0, s1);
@@ -944,7 +947,7 @@ struct TreePlan {
 };
 
 // The tcgen05 kernel takes head dims 64 and 128 and trees whose bitmaps it holds (and
-// lists and grids whose counts fit in an int), from a single row on: even trees of 5 over 2.2 GB of K/V take 335 us there and 403 us in
+// lists and grids whose counts fit in an int), from a single row on: even trees of 5 over 2.2 GB of K/V take 340 us there and took 403 us in
 // the mma.sync kernel, which serves everything else.
 static TreePlan tree_plan(int B, int Hq, int Hkv, int T, int d, int block_size, int max_blocks,
                           int split_tokens) {
