@@ -600,7 +600,9 @@ __global__ void __launch_bounds__(kPagedWarps * 32)
     if constexpr (TREE) {
       // A node's V row that holds NaN or infinity must not reach the rows that do
       // not see it, and 0 x NaN in the MMA below would: such rows (none, as a rule)
-      // are added here for the rows that see them and then zeroed in the tile.
+      // are added here for the rows that see them and then zeroed in the tile. Their
+      // P is made again in fp32 from the scores: a half of it would lose bits in the
+      // row's finite columns, and as fp16 a small one would be 0, and 0 x inf NaN.
       if (need_mask) {
         uint32_t bad = 0;  // lane's share: 16-bit elements whose exponent is all ones
         for (int q = lane; q < kTileTok * KC; q += 32) {
@@ -620,11 +622,13 @@ __global__ void __launch_bounds__(kPagedWarps * 32)
           for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
-              // P of (row, key j) sits in lane (row's quad) + (j % 8) / 2
+              // the score of (row, key j) sits in lane (row's quad) + (j % 8) / 2
               const int src = (lane & ~3) | ((j & 7) >> 1);
-              const uint32_t pw = __shfl_sync(0xffffffffu, j < 8 ? pa[mt][hf] : pa[mt][2 + hf], src);
-              const float2 pf = unpack2<BF16>(pw);
-              const float pj = (j & 1) ? pf.y : pf.x;
+              const float lo = j < 8 ? s[mt][0][2 * hf] : s[mt][1][2 * hf];
+              const float hi = j < 8 ? s[mt][0][2 * hf + 1] : s[mt][1][2 * hf + 1];
+              const float sj = __shfl_sync(0xffffffffu, (j & 1) ? hi : lo, src);
+              const float m_use = m_run[mt][hf] == -INFINITY ? 0.f : m_run[mt][hf];
+              const float pj = ex2(sj * p.scale_log2 - m_use);
               if ((win[mt][hf] >> j) & 1u) {
 #pragma unroll
                 for (int nt = 0; nt < D / 8; ++nt) {
