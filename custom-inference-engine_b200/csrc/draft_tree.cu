@@ -49,6 +49,11 @@ constexpr int kVfWarps = kVfThreads / 32;
 constexpr int kSeg = 512;         // elements of a row summed by one warp at a time; one per
                                   // thread when the drawn token is looked for in it
 constexpr int kVfMaxCluster = 8;  // portable cluster size
+constexpr int kVfMaxRow = 1 << 23;  // elements of a row
+// shared memory of a CTA for rows of `segs` segments of its own and T nodes
+constexpr size_t vf_smem_bytes(int segs, int T) {
+  return static_cast<size_t>(segs) * 8 + static_cast<size_t>(T) * (8 + 6 * 4);
+}
 static_assert(kSeg == kVfThreads, "the search gives every thread one element");
 
 struct VerifyParams {
@@ -507,9 +512,12 @@ static int launch_verify(const VerifyParams& prm, int B, int cl, size_t smem, cu
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
+  // the limit belongs to the kernel, not to this call: one value for every caller, so
+  // that no thread lowers it between another's setting and its launch
   if (smem > 40000)
-    cudaFuncSetAttribute(verify_kernel<T, VEC, GREEDY>,
-                         cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    cudaFuncSetAttribute(
+        verify_kernel<T, VEC, GREEDY>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        static_cast<int>(vf_smem_bytes(kVfMaxRow / kSeg / kVfMaxCluster, CIE_MAX_TREE)));
   const cudaError_t e = cudaLaunchKernelEx(&cfg, verify_kernel<T, VEC, GREEDY>, prm);
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -622,7 +630,7 @@ extern "C" int cie_verify_drafts(const void* tokens, int64_t tokens_stride_b, in
                 "cie_verify_drafts: null pointer");
   CIE_CHECK_ARG(B >= 0 && T > 0 && V > 0, "cie_verify_drafts: bad shape");
   CIE_CHECK_ARG(T <= CIE_MAX_TREE, "cie_verify_drafts: %d nodes, at most %d", T, CIE_MAX_TREE);
-  CIE_CHECK_ARG(V <= (1 << 23), "cie_verify_drafts: %d tokens in a row, at most %d", V, 1 << 23);
+  CIE_CHECK_ARG(V <= kVfMaxRow, "cie_verify_drafts: %d tokens in a row, at most %d", V, kVfMaxRow);
   CIE_CHECK_ARG(dtype == CIE_DTYPE_BF16 || dtype == CIE_DTYPE_FP16 || dtype == CIE_DTYPE_FP32,
                 "cie_verify_drafts: bad dtype %d", dtype);
   CIE_CHECK_ARG(draft == nullptr || (draft_strides && draft_rows > 0 && draft_rows <= T),
@@ -665,7 +673,7 @@ extern "C" int cie_verify_drafts(const void* tokens, int64_t tokens_stride_b, in
   prm.T = T;
   prm.V = V;
   prm.segs = (nseg + cl - 1) / cl;
-  const size_t smem = static_cast<size_t>(prm.segs) * 8 + static_cast<size_t>(T) * (8 + 6 * 4);
+  const size_t smem = vf_smem_bytes(prm.segs, T);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   switch (dtype) {
     case CIE_DTYPE_BF16: return dispatch_verify<__nv_bfloat16>(prm, B, cl, smem, vec, st);

@@ -142,7 +142,7 @@ __host__ __device__ constexpr int paged_smem_bytes() {
 // Tree mode, behind the shared memory of paged_smem_bytes: M parents, RG depths
 // and RG ancestor bitmaps.
 __host__ __device__ constexpr int tree_words(int M) { return (M + 31) / 32; }
-static int tree_smem_bytes(int M, int rg_rows) { return 4 * (M + rg_rows * (1 + tree_words(M))); }
+constexpr int tree_smem_bytes(int M, int rg_rows) { return 4 * (M + rg_rows * (1 + tree_words(M))); }
 
 template <int D, int MT, bool BF16, bool PAGED, bool TMA, bool TREE>
 __global__ void __launch_bounds__(kPagedWarps * 32)
@@ -901,8 +901,12 @@ template <int D, int MT, bool BF16, bool PAGED, bool TMA, bool TREE>
 static int launch_mma_t(const CUtensorMap& mk, const CUtensorMap& mv, const PagedParams& prm,
                         cudaStream_t st) {
   const int smem = paged_smem_bytes<D, MT>() + (TREE ? tree_smem_bytes(prm.M, 16 * MT) : 0);
+  // the limit belongs to the kernel, not to this call: always the same value, so that a
+  // thread with a smaller tree cannot lower it between another's setting and its launch
+  constexpr int most = paged_smem_bytes<D, MT>() + (TREE ? tree_smem_bytes(CIE_MAX_TREE, 16 * MT) : 0);
+  static_assert(most <= 227 * 1024, "shared memory of the largest tree");
   auto kern = paged_attn_kernel<D, MT, BF16, PAGED, TMA, TREE>;
-  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
   dim3 grid(prm.max_splits, prm.Hkv * prm.row_groups, prm.B);
   kern<<<grid, kPagedWarps * 32, smem, st>>>(mk, mv, prm);
   CIE_CHECK_LAUNCH("paged_attn_kernel");
