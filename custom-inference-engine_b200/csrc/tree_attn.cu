@@ -968,10 +968,22 @@ static TreePlan tree_plan(int B, int Hq, int Hkv, int T, int d, int block_size, 
   const int slots = num_sms() * 2;  // CTAs that run at once
   tp.min_run = kTcMinRun;
   tp.whole = kTcWhole;
-  // parts of a head group's list: the slots over the groups; with so many groups that
-  // more than a tenth of the slots would idle, three waves of CTAs
+  // parts of a head group's list: as many as run at once. With so many groups that more
+  // than a tenth of the slots would idle, two to four rounds of CTAs, whichever leaves a
+  // slot the smallest share of a list (rounds / parts). 8 contexts of 4K-8K, d = 64, one, two
+  // and three rounds: 64 groups 186, 173 and 182 us; 80 groups 243, 214 and 215; 100 groups
+  // 356, 292 and 281. One part more is a round more: 200, 243 and 309 us.
   int64_t parts = slots / groups;
-  if (parts == 0 || (slots - parts * groups) * 10 > slots) parts = (3 * slots + groups - 1) / groups;
+  if (parts == 0 || (slots - parts * groups) * 10 > slots) {
+    int64_t rounds = 1;
+    for (int r = 2; r <= 4; ++r) {
+      const int64_t n = static_cast<int64_t>(r) * slots / groups;
+      if (n > 0 && (parts == 0 || r * parts < rounds * n)) {
+        parts = n;
+        rounds = r;
+      }
+    }
+  }
   if (split_tokens > 0) {  // runs of that many tokens
     tp.min_run = (split_tokens + kTcKeys - 1) / kTcKeys;
     tp.whole = tp.min_run;
