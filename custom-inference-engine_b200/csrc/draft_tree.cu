@@ -9,7 +9,10 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
+#include <memory>
+#include <new>
 #include <type_traits>
 
 #include "cie_common.cuh"
@@ -615,6 +618,26 @@ __global__ void __launch_bounds__(kKeepThreads) keep_path_kernel(const __grid_co
   }
 }
 
+// The index in `pools` of a pool that shares memory with another, each `bytes` long; -1:
+// none, -2: no host memory to look for it. The moves of two such pools would race.
+static int shared_pool(void* const* pools, int n, uint64_t bytes) {
+  uintptr_t few[kMaxPools];
+  std::unique_ptr<uintptr_t[]> many;
+  uintptr_t* at = few;
+  if (n > kMaxPools) {
+    many.reset(new (std::nothrow) uintptr_t[n]);
+    at = many.get();
+    if (at == nullptr) return -2;
+  }
+  for (int i = 0; i < n; ++i) at[i] = reinterpret_cast<uintptr_t>(pools[i]);
+  std::sort(at, at + n);
+  for (int i = 1; i < n; ++i)
+    if (at[i] - at[i - 1] < bytes)
+      for (int k = n - 1; k >= 0; --k)
+        if (reinterpret_cast<uintptr_t>(pools[k]) == at[i]) return k;
+  return -1;
+}
+
 }  // namespace cie
 
 using namespace cie;
@@ -702,6 +725,10 @@ extern "C" int cie_keep_path(void* const* pools, int n_pools, const int32_t* blo
                   "cie_keep_path: pool %d null or not 16-byte aligned", i);
   if (B == 0) return CIE_OK;
   CIE_CHECK_ARG(B <= 65535, "cie_keep_path: B must be <= 65535");
+  const int twice =
+      shared_pool(pools, n_pools, static_cast<uint64_t>(num_blocks) * block_size * row_bytes);
+  CIE_CHECK_ARG(twice != -2, "cie_keep_path: no host memory for %d pools", n_pools);
+  CIE_CHECK_ARG(twice == -1, "cie_keep_path: pool %d shares memory with another", twice);
   for (int p0 = 0; p0 == 0 || p0 < n_pools; p0 += kMaxPools) {
     KeepParams prm{};
     prm.n_pools = n_pools - p0 < kMaxPools ? n_pools - p0 : kMaxPools;

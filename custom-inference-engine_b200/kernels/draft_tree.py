@@ -295,7 +295,7 @@ def keep_path(
     """Move the kept nodes' rows to the slots behind the history, in place.
 
     pools: the K and V pools of every layer, each (num_blocks, block_size, Hkv, D),
-    all of one shape and dtype. kv_lens: int32 (B,), counting the T nodes. path:
+    all of one shape and dtype, none of them twice. kv_lens: int32 (B,), counting the T nodes. path:
     int32 (B, T) and n: int32 (B,) as ``verify_drafts`` returns them. Slot
     base + i takes the row of slot base + path[b, i] for i < n[b], where
     base = kv_lens[b] - T. Rows elsewhere stay as they are. Returns the new

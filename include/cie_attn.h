@@ -324,7 +324,8 @@ int cie_verify_drafts(const void* tokens, int64_t tokens_stride_b,
  * array of n_pools device pointers, each to num_blocks * block_size rows of
  * row_bytes bytes (a multiple of 16). path rises, as cie_verify_drafts gives it;
  * an entry below its index or beyond T is skipped and sets CIE_DEV_BAD_TREE. One
- * launch per 256 pools. Two sequences must not share a block that is written.
+ * launch per 256 pools. No two pools may share memory (refused), and two sequences must
+ * not share a block that is written.
  */
 int cie_keep_path(void* const* pools, int n_pools, const int32_t* block_tables,
                   const int32_t* kv_lens, const int32_t* path, const int32_t* n,
