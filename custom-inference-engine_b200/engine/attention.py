@@ -194,7 +194,8 @@ def end_tree_step(cache: PagedKVCache, step: BatchStep, verdict) -> list[list[in
 
     The kept nodes' K/V move behind each history, in all layers, and the tables shrink
     to them. Returns each sequence's new tokens; the last is not in the cache yet and is
-    the root of the next tree. Reading them is the step's only host sync.
+    the root of the next tree. Reading them is the step's only host sync. A step ends
+    once, with its tables as it left them.
     """
     if step.parents is None:
         raise ValueError("end_tree_step ends a step that begin_step began with parents")
@@ -202,6 +203,8 @@ def end_tree_step(cache: PagedKVCache, step: BatchStep, verdict) -> list[list[in
     if verdict.path.shape != (B, T) or verdict.tokens.shape != (B, T):
         raise ValueError(f"the verdict is for {tuple(verdict.path.shape)} (sequences, nodes), "
                          f"the step for ({B}, {T})")
+    if any(t.length != s + T for t, s in zip(step.tables, step.starts)):
+        raise ValueError("the step has ended, or its tables have changed since it began")
     cache.keep_path(step.block_tables, step.kv_lens, verdict.path, verdict.n)
     both = torch.cat([verdict.n[:, None].to(verdict.tokens.dtype), verdict.tokens], 1).tolist()
     for table, start, row in zip(step.tables, step.starts, both):

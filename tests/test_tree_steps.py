@@ -1,0 +1,64 @@
+"""CPU checks of the engine's steps over trees of drafts: what they refuse, with nothing changed by it."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from engine.cache.allocator import BlockAllocator
+from engine.cache.kv_cache import pack_tables
+
+
+class HostCache:
+    """The host side of a PagedKVCache; moves on the device are counted only."""
+
+    device = torch.device("cpu")
+
+    def __init__(self, num_blocks=32, block_size=4):
+        self.alloc = BlockAllocator(num_blocks, block_size)
+        self.moves = 0
+
+    def device_tables(self, tables):
+        return pack_tables(tables, "cpu")
+
+    def keep_path(self, block_tables, kv_lens, path, n):
+        self.moves += 1
+
+    def rollback(self, table, new_length):
+        self.alloc.rollback(table, new_length)
+
+
+def state(cache, tables):
+    return [(t.length, list(t.blocks)) for t in tables], list(cache.alloc._free)
+
+
+def verdict(*rows, T):
+    """Each row: the new tokens of a sequence."""
+    from kernels.draft_tree import Verdict
+
+    n = [len(r) for r in rows]
+    pad = [r + [-1] * (T - len(r)) for r in rows]
+    path = [list(range(k)) + [-1] * (T - k) for k in n]
+    return Verdict(torch.tensor(pad), torch.tensor(path, dtype=torch.int32), torch.tensor(n, dtype=torch.int32))
+
+
+def test_a_tree_step_ends_once():
+    """Ending a step moves rows within the cache: a second time, or after the tables changed, the rows it
+    would take have been overwritten or belong to something else."""
+    from engine.attention import begin_step, end_tree_step
+
+    cache = HostCache()
+    tables = [cache.alloc.new_sequence() for _ in range(2)]
+    step = begin_step(cache, tables, 5, parents=[-1, 0, 0, 1, 2])
+    v = verdict([7, 8, 9], [4], T=5)
+    assert end_tree_step(cache, step, v) == [[7, 8, 9], [4]] and [t.length for t in tables] == [3, 1]
+    was = state(cache, tables)
+    with pytest.raises(ValueError, match="ended"):
+        end_tree_step(cache, step, v)
+    assert cache.moves == 1 and state(cache, tables) == was
+    step = begin_step(cache, tables, 5, parents=[-1, 0, 0, 1, 2])
+    cache.rollback(tables[1], 2)
+    was = state(cache, tables)
+    with pytest.raises(ValueError, match="ended"):
+        end_tree_step(cache, step, v)
+    assert cache.moves == 1 and state(cache, tables) == was
