@@ -169,6 +169,11 @@ def begin_step(cache: PagedKVCache, tables: list[BlockTable], new_tokens: int,
     if new_tokens <= 0:
         raise ValueError(f"new_tokens must be positive, got {new_tokens}")
     if parents is not None:
+        from kernels import _lib
+
+        # whatever the layers would refuse, before the tables change
+        if new_tokens > _lib.CIE_MAX_TREE:
+            raise ValueError(f"a tree of {new_tokens} nodes, at most {_lib.CIE_MAX_TREE}")
         if not (isinstance(parents, torch.Tensor) and parents.is_cuda):
             parents = _tree_parents(parents, len(tables), new_tokens)
             parents = _to_device(parents, cache.device)
@@ -177,6 +182,8 @@ def begin_step(cache: PagedKVCache, tables: list[BlockTable], new_tokens: int,
             raise ValueError(f"parents must be int32 ({new_tokens},) or "
                              f"({len(tables)}, {new_tokens}), got {parents.dtype} "
                              f"{tuple(parents.shape)}")
+        elif parents.device != torch.device(cache.device):
+            raise RuntimeError("begin_step requires parents and cache on one CUDA device")
     starts = [t.length for t in tables]
     for t, s in zip(tables, starts):
         cache.alloc.reserve(t, s + new_tokens)

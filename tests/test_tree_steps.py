@@ -62,3 +62,33 @@ def test_a_tree_step_ends_once():
     with pytest.raises(ValueError, match="ended"):
         end_tree_step(cache, step, v)
     assert cache.moves == 1 and state(cache, tables) == was
+
+
+@pytest.mark.parametrize("what", ["nodes", "device"])
+def test_begin_step_refuses_before_it_reserves(what):
+    """Trees that no kernel takes are refused while the tables are as they were, not by the first layer."""
+    from engine.attention import begin_step
+
+    cache = HostCache(num_blocks=600)
+    tables = [cache.alloc.new_sequence()]
+    was = state(cache, tables)
+    if what == "nodes":
+        with pytest.raises(ValueError, match="at most 1024"):
+            begin_step(cache, tables, 1025, parents=[-1] * 1025)
+    else:
+        parents = FakeCudaTensor(torch.tensor([-1, 0, 0], dtype=torch.int32))
+        cache.device = torch.device("cuda", 1)
+        with pytest.raises(RuntimeError, match="one CUDA device"):
+            begin_step(cache, tables, 3, parents=parents)
+    assert state(cache, tables) == was
+
+
+class FakeCudaTensor(torch.Tensor):
+    """An int32 host tensor that says it is on the first GPU."""
+
+    @staticmethod
+    def __new__(cls, t):
+        return t.as_subclass(cls)
+
+    is_cuda = True
+    device = torch.device("cuda", 0)
