@@ -174,6 +174,8 @@ def begin_step(cache: PagedKVCache, tables: list[BlockTable], new_tokens: int,
         # whatever the layers would refuse, before the tables change
         if new_tokens > _lib.CIE_MAX_TREE:
             raise ValueError(f"a tree of {new_tokens} nodes, at most {_lib.CIE_MAX_TREE}")
+        if len({id(t) for t in tables}) != len(tables):
+            raise ValueError("a step over trees holds a sequence twice")
         if not (isinstance(parents, torch.Tensor) and parents.is_cuda):
             parents = _tree_parents(parents, len(tables), new_tokens)
             parents = _to_device(parents, cache.device)

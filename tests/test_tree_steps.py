@@ -92,3 +92,16 @@ class FakeCudaTensor(torch.Tensor):
 
     is_cuda = True
     device = torch.device("cuda", 0)
+
+
+def test_begin_step_takes_a_sequence_once():
+    """Two trees in the same slots of one sequence would overwrite each other and end twice."""
+    from engine.attention import begin_step
+
+    cache = HostCache()
+    a, b = cache.alloc.new_sequence(), cache.alloc.new_sequence()
+    was = state(cache, [a, b])
+    with pytest.raises(ValueError, match="twice"):
+        begin_step(cache, [a, b, a], 3, parents=[-1, 0, 0])
+    assert state(cache, [a, b]) == was
+    assert begin_step(cache, [a, b], 3, parents=[-1, 0, 0]).starts == [0, 0]  # equal, but two sequences
