@@ -143,14 +143,16 @@ class BatchStep:
 def _tree_parents(parents, batch: int, nodes: int) -> torch.Tensor:
     """int32 (nodes,) or (batch, nodes) from lists, checked: node 0 the root, every
     other node's parent below it, -1 for padding."""
-    t = torch.as_tensor(parents, dtype=torch.int32)
+    t = torch.as_tensor(parents)
+    if t.dtype not in (torch.int64, torch.int32, torch.int16, torch.int8):
+        raise ValueError(f"parents must be whole numbers, got {t.dtype}")
     if t.shape != (nodes,) and t.shape != (batch, nodes):
         raise ValueError(f"parents must be ({nodes},) or ({batch}, {nodes}), got "
                          f"{tuple(t.shape)}")
-    at = torch.arange(nodes, dtype=torch.int32)
+    at = torch.arange(nodes)
     if bool((t >= at).any()) or bool((t < -1).any()):
         raise ValueError("a node's parent must be an earlier node, or -1")
-    return t
+    return t.to(torch.int32)
 
 
 def begin_step(cache: PagedKVCache, tables: list[BlockTable], new_tokens: int,

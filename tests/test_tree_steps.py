@@ -105,3 +105,25 @@ def test_begin_step_takes_a_sequence_once():
         begin_step(cache, [a, b, a], 3, parents=[-1, 0, 0])
     assert state(cache, [a, b]) == was
     assert begin_step(cache, [a, b], 3, parents=[-1, 0, 0]).starts == [0, 0]  # equal, but two sequences
+
+
+@pytest.mark.parametrize("parents", [[-1, 0, 0.5], [-1.0, 0.0, 1.0], torch.tensor([-1, 0, 2 ** 32]), torch.tensor([-1, 0, -1 - 2 ** 32]),
+                                     torch.tensor([True, False, False]), [-1, 0, 2 ** 40]])
+def test_begin_step_takes_whole_numbers_in_range(parents):
+    """Nothing is cut to an index that it is not: fractions and numbers beyond 32 bits are refused."""
+    from engine.attention import begin_step
+
+    cache = HostCache()
+    tables = [cache.alloc.new_sequence()]
+    with pytest.raises(ValueError, match="parent"):
+        begin_step(cache, tables, 3, parents=parents)
+    assert state(cache, tables) == state(HostCache(), [HostCache().alloc.new_sequence()])
+
+
+@pytest.mark.parametrize("kind", [torch.int64, torch.int32, torch.int8, torch.int16])
+def test_begin_step_takes_any_kind_of_whole_number(kind):
+    from engine.attention import begin_step
+
+    cache = HostCache()
+    step = begin_step(cache, [cache.alloc.new_sequence()], 3, parents=torch.tensor([[-1, 0, 1]], dtype=kind))
+    assert step.parents.dtype == torch.int32 and step.parents.tolist() == [[-1, 0, 1]]
