@@ -325,6 +325,14 @@ def rope_append(
         raise ValueError("rope_append expects one FP16/BF16 dtype for all tensors")
     if block_tables.dtype != torch.int32 or start_pos.dtype != torch.int32:
         raise ValueError("block_tables and start_pos must be int32")
+    if parents is not None:
+        if block_tables.ndim != 2 or block_tables.shape[0] != B or start_pos.shape != (B,):
+            raise ValueError("block_tables must be (B, max_blocks) and start_pos (B,)")
+        if not (k_pool.is_contiguous() and v_pool.is_contiguous()):
+            raise ValueError("k_pool/v_pool must be contiguous")
+        if {t.get_device() for t in (v_new, k_pool, v_pool, block_tables, start_pos)} != {
+                k_new.get_device()}:
+            raise RuntimeError("rope_append requires all tensors on one CUDA device")
     lib = _require()
     k_new = _kernel_ready(k_new)
     v_new = _kernel_ready(v_new)
