@@ -842,6 +842,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
         ++pieces;
         if (ahead.more) hand_over(ahead, pieces);
       }
+      cp_async_wait<0>();  // a role gave up: the next piece's Q and parents may be on their way
       if (!ok) raise_status(CIE_DEV_TIMEOUT);
     }
   }
