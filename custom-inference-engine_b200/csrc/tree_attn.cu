@@ -121,6 +121,19 @@ __device__ __forceinline__ TcPlan tc_plan(const PagedParams& p, int keys, int pa
   return plan;
 }
 
+// The first sequence with keys among b, b + by, b + 2 by, .., B when there is none: 32 at a
+// time, as a padded batch may have hundreds of idle sequences in a row. Not inlined: the
+// roles' code, which all CTAs fetch, stays short (inlined, 1 us of 29 in a batch without any).
+__device__ __noinline__ int tc_skip_idle(const int32_t* kv_lens, int B, int b, int by) {
+  const int lane = threadIdx.x & 31;
+  for (; b < B; b += 32 * by) {
+    const int i = b + lane * by;
+    const uint32_t hit = __ballot_sync(0xffffffffu, i < B && kv_lens[i] > 0);
+    if (hit) return b + (__ffs(hit) - 1) * by;
+  }
+  return B;
+}
+
 // A CTA's walk over its pieces of sequences. All members are warp-uniform.
 struct TcWalk {
   int b, kv_len, tiles;  // sequence, its length and key tiles
@@ -132,29 +145,29 @@ struct TcWalk {
     kv_len = tc_len(p, b);
     tiles = (kv_len + keys - 1) / keys;
   }
+  // the first sequence with keys from b on, in steps of `by`
+  __device__ __forceinline__ bool busy(const PagedParams& p, int keys, int by) {
+    while (b < p.B) {
+      seq(p, keys);
+      if (tiles > 0) return true;
+      b = tc_skip_idle(p.kv_lens, p.B, b + by, by);
+    }
+    return false;
+  }
   // the first piece of the run in sequence b or behind it
   __device__ __forceinline__ void find(const PagedParams& p, int keys) {
-    for (; b < p.B && at < hi; ++b) {
-      seq(p, keys);
-      if (tiles > 0) {
-        first = max(lo - at - kTcOpen, 0);
-        n = min(hi - at - kTcOpen, tiles) - first;
-        if (n > 0) return;
-      }
+    for (; at < hi && busy(p, keys, 1); ++b) {
+      first = max(lo - at - kTcOpen, 0);
+      n = min(hi - at - kTcOpen, tiles) - first;
+      if (n > 0) return;
       at += tc_places(tiles);
     }
     more = false;
   }
   // whole sequences: the first with keys from b on, in steps of the parts
   __device__ __forceinline__ void deal(const PagedParams& p, int keys) {
-    for (; b < p.B; b += hi) {
-      seq(p, keys);
-      if (tiles > 0) {
-        n = tiles;
-        return;
-      }
-    }
-    more = false;
+    more = busy(p, keys, hi);
+    n = tiles;
   }
   __device__ __forceinline__ void start(const PagedParams& p, int keys, int groups, int lane,
                                         int len) {
@@ -871,10 +884,14 @@ __global__ void __launch_bounds__(kTcMergeThreads)
   const int lane = threadIdx.x & 31;
   const int groups = p.Hkv * p.row_groups;
   const int b = blockIdx.x / groups, y = blockIdx.x % groups;
+  const int tiles = (tc_len(p, b) + keys - 1) / keys;
+  if (tiles == 0) {  // idle: nothing to plan for
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
   int mine;
   const TcPlan plan =
       tc_plan(p, keys, ctas / groups, lane, lane < p.B ? tc_len(p, lane) : 0, mine);
-  const int tiles = (tc_len(p, b) + keys - 1) / keys;
   int at = 0;  // the sequence's place in the list
   if (lane < b) at = mine;
   for (int i = lane + 32; i < b; i += 32) at += tc_places((tc_len(p, i) + keys - 1) / keys);
@@ -883,7 +900,7 @@ __global__ void __launch_bounds__(kTcMergeThreads)
   // The partial results are there. Every CTA waits, also one without work: what
   // follows this kernel on the stream may count on the whole call being done.
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (plan.whole || tiles == 0 || c0 == c1) return;
+  if (plan.whole || c0 == c1) return;
   const int r = blockIdx.y * ROWS + threadIdx.x / D4, c = threadIdx.x % D4;
   const int gr = (y % p.row_groups) * p.rg_rows + r;
   if (r >= p.rg_rows || gr >= p.G * p.M) return;
