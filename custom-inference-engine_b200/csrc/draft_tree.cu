@@ -570,12 +570,14 @@ __global__ void __launch_bounds__(kKeepThreads) keep_path_kernel(const __grid_co
   __shared__ int2 s_move[CIE_MAX_TREE];  // (from, to) pool rows; from < 0: nothing to do
   const int b = blockIdx.y;
   int n = p.n[b];
-  const int base = p.kv_lens[b] - p.T;
+  const int len = max(p.kv_lens[b], 0);
+  const int base = len - p.T;
   const int tid = threadIdx.x;
   if (n < 0 || n > p.T) {
     if (tid == 0) raise_status(CIE_DEV_BAD_TREE);
     n = n < 0 ? 0 : p.T;
   }
+  if (len == 0) n = 0;  // an idle slot of a padded batch has no rows, whatever its verdict
   const int32_t* table = p.tables + static_cast<int64_t>(b) * p.max_blocks;
   auto row_of = [&](int pos) -> int {
     const int lb = pos / p.block_size;

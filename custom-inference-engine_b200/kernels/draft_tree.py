@@ -298,7 +298,8 @@ def keep_path(
     all of one shape and dtype, none of them twice. kv_lens: int32 (B,), counting the T nodes. path:
     int32 (B, T) and n: int32 (B,) as ``verify_drafts`` returns them. Slot
     base + i takes the row of slot base + path[b, i] for i < n[b], where
-    base = kv_lens[b] - T. Rows elsewhere stay as they are. Returns the new
+    base = kv_lens[b] - T; nothing of an idle sequence (kv_lens[b] = 0) moves. Rows
+    elsewhere stay as they are. Returns the new
     lengths, max(0, base + n[b]), int32 (B,).
     """
     index = path.get_device()

@@ -320,7 +320,8 @@ int cie_verify_drafts(const void* tokens, int64_t tokens_stride_b,
  * Moves the kept nodes' K and V rows behind the history, in every pool, in
  * place: for 1 <= i < n[b]
  *   pool[slot base + i] = pool[slot base + path[b, i]],  base = kv_lens[b] - T
- * and new_lens[b] = max(0, base + n[b]) (new_lens may be NULL). pools: host
+ * and new_lens[b] = max(0, base + n[b]) (new_lens may be NULL). A sequence with
+ * kv_lens[b] = 0 is idle: nothing moves and its length stays 0. pools: host
  * array of n_pools device pointers, each to num_blocks * block_size rows of
  * row_bytes bytes (a multiple of 16). path rises, as cie_verify_drafts gives it;
  * an entry below its index or beyond T is skipped and sets CIE_DEV_BAD_TREE. One
