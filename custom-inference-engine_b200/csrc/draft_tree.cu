@@ -1,7 +1,7 @@
 // draft_tree.cu — the two steps that follow the attention over a tree of drafted
 // tokens: which nodes are kept (verify_drafts) and the move of their K/V rows
 // behind the history (keep_path). The attention itself is cie_tree_attn in
-// paged_attn.cu. The reference decodes greedily on the host with one chain
+// tree_attn.cu. The reference decodes greedily on the host with one chain
 // (engine/decode/speculative.py:88-123); here a whole batch of trees is decided
 // on the device, without a host sync.
 #include <cooperative_groups.h>

@@ -37,8 +37,8 @@
 // the head dims and tree sizes that tree_attn.cu does not (d 16, 32 and 256, more
 // than 256 nodes); more than 32 rows per kv head (64 at d <= 64) read K/V again for
 // every group of rows: 776 us for trees of 16 over 2.2 GB of K/V at d = 128, where
-// the tcgen05 kernel took 350 (P rounded once in both). P in two halves: 73 against 69 us
-// for 16 rows at d = 256, 436 against 400 us for 256 rows at d = 32.
+// the tcgen05 kernel took 350 (P rounded once in both). P in two halves costs 73 against
+// 68 us for 16 rows at d = 256, 953 against 887 us for 256, nothing at d = 32 (400 us).
 #include <cuda.h>
 #include <cuda_runtime.h>
 

@@ -34,11 +34,12 @@
 // SM's share of HBM; its MMAs take 960 and its exponentials 512 cycles (MUFU). Two
 // CTAs share an SM (256 TMEM columns, ~100 KB each), so one's hand-offs hide behind
 // the other's. More than 128 rows take another pass over K/V, which comes from L2.
-// Measured on B200 (2.2 GB of K/V, 32 contexts of 1K-32K, d = 128, bf16): trees of 5
-// 340 us (6.5 TB/s), of 16 371 us (6.0 TB/s), of 32 422 us (5.3 TB/s); with P rounded
-// once 328, 346 and 375 us. Trees of 64 over 8 contexts of up to 16K (256 rows) 112 us,
-// with P rounded once 98; so measured, a form with two 128-row tiles in one CTA that
-// fills the SM by itself took 103.
+// Measured on B200 (2.2 GB of K/V, 32 contexts of 1K-32K, d = 128, bf16; on two GPUs):
+// trees of 5 340-357 us (6.2-6.5 TB/s), of 16 371-394 us (5.6-6.0), of 32 422-449 us
+// (5.0-5.3); with P rounded once 328-336, 346-356 and 375-390 us. For seconds on end,
+// under the power cap, trees of 16 take 451 us, with P rounded once 396. Trees of 64 over
+// 8 contexts of up to 16K (256 rows) 112-115 us, with P rounded once 98; so measured, a
+// form with two 128-row tiles in one CTA that fills the SM by itself took 103.
 //
 // The choices below were measured with P rounded once to bf16.
 #include <cuda.h>

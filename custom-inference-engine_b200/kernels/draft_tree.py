@@ -214,8 +214,9 @@ def verify_drafts(
     The children x of a node with rows p and q are tested in index order: kept if
     u q(x) m < r(x), where r = p and m = 1 at first; otherwise r becomes
     max(r - m q, 0) and m its sum. If no child is kept the last token is drawn
-    from r by its cumulative sum. The kept tokens are then distributed as if drawn
-    from the target alone. Without ``uniforms`` the walk is greedy: the child that
+    from r by its cumulative sum. For rows that sum to 1 the kept tokens are then
+    distributed as if drawn from the target alone (16-bit rows: to their rounding; rows
+    cut to their likeliest tokens must be normalised again). Without ``uniforms`` the walk is greedy: the child that
     drafted the row's largest entry (the lowest such index) is kept; rows may then be
     logits.
 

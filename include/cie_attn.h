@@ -285,7 +285,8 @@ size_t cie_tree_attn_workspace(int B, int Hq, int Hkv, int T, int d,
  *             last token that was kept before
  *   parents:  as above; node 0 is the root
  *   target:   (B, T, V) in dtype (any cie_dtype): row i is the target model's
- *             distribution after node i. strides: B and T dims, elements.
+ *             distribution after node i, which sums to 1 (m below begins with it).
+ *             strides: B and T dims, elements.
  *   draft:    NULL, or (B, draft_rows, V): row i is the distribution that the
  *             children of node i were drawn from, independently of one another.
  *             Nodes from draft_rows on are leaves. NULL: the children were
